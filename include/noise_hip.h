@@ -507,6 +507,69 @@ typedef struct noise_adam_tensor {
 int noise_adam_batch(const noise_adam_tensor_t* tensors, int n, float beta1, float beta2, float eps,
                      noise_stream_t stream);
 
+/* ---------------------------------------------------------------- serving: prompts, and a key / value cache
+ * No counterpart in the reference, which trains and scores; this is what answering with a trained model needs next to
+ * it. Rows are packed: `rows` rows of `sequences` sequences, sequence b owning rows starts[b] .. starts[b + 1] (int32,
+ * [sequences + 1], nondecreasing; rows outside starts[0] .. starts[sequences] belong to none). A query at position s sees key
+ * j when 0 <= j <= s and (s - j <= window or j < sinks); pass INT_MAX for no window. A row that sees no key is zero; keys and
+ * values that a row does not see take no part in it, whatever they hold. dim is 64 or 128, heads a multiple of kv_heads,
+ * query head h reading kv head h / (heads / kv_heads). */
+#define NOISE_ROWS_BF16 0
+#define NOISE_ROWS_F16 1
+#define NOISE_ROWS_F32 2 /* rows written into the cache or read out of it only */
+
+/* y = softmax(scale q k^T) v of whole sequences. q [rows, heads, dim], k and v [rows, kv_heads, dim] of `type` (NOISE_ROWS_BF16
+ * or F16): row r's head h at r * ld + h * hs elements (multiples of 8; pointers 16-byte aligned). starts null: sequences of T
+ * rows each, rows = sequences * T. y [rows, heads, dim] of the same type, contiguous. Rows of no sequence are set to zero
+ * (fill != 0) or left as they were. */
+int noise_sink_attention(const void* q, long q_ld, long q_hs, const void* k, long k_ld, long k_hs, const void* v, long v_ld,
+                         long v_hs, const int* starts, int sequences, int rows, int T, int heads, int kv_heads, int dim,
+                         int type, int window, int sinks, float scale, void* y, int fill, noise_stream_t stream);
+
+/* A paged cache of keys and values in microscaled floating point. Token t of page g, kv head h holds its dim channels as
+ * codes (keys / values [pages, kv_heads, page_size, dim / 2 or dim] bytes, 16-byte aligned) and one byte e per 32 channels
+ * (scales [pages, kv_heads, page_size, dim / 32], 4-byte aligned): value = code * 2^(e - 127), NaN where e is 255. page_size is
+ * a power of two, 16 .. 256. */
+#define NOISE_CACHE_FP4 0 /* e2m1: two codes to a byte, the even channel in the low half */
+#define NOISE_CACHE_FP8 1 /* e4m3: a byte a code */
+typedef struct noise_cache {
+  void *keys, *key_scales, *values, *value_scales;
+  long pages;
+  int page_size, kv_heads, dim, format;
+} noise_cache_t;
+
+/* The rows of a call: the m rows of sequence b sit at positions lengths[b] - m .. lengths[b] - 1 (the newest tokens of a
+ * sequence that holds lengths[b]); starts null: one row a sequence. Position p of sequence b is token p % page_size of
+ * page table[b * table_ld + p / page_size] (int32, table_pages entries a sequence). Rows of no sequence and rows at negative
+ * positions are at no place; a page outside [0, pages), or a position past the table, is a bad place. */
+typedef struct noise_sequences {
+  const int* table;
+  long table_ld;
+  int table_pages;
+  const int* lengths;
+  const int* starts;
+  int sequences, rows;
+} noise_sequences_t;
+
+/* Quantises k and v [rows, kv_heads, dim] of `type` into the rows' places; rows at no place or a bad one are dropped. Per 32
+ * channels: e - 127 is the smallest integer in -127 .. 127 with max|x| <= MAX 2^(e - 127) (MAX 6 or 448), the codes the
+ * nearest of x 2^(127 - e), ties to even; a group with an infinity or NaN gets e = 255. The rows' places must be distinct.
+ * Both structs are host memory, read before the call returns. */
+int noise_cache_write(const noise_cache_t* cache, const noise_sequences_t* seqs, const void* k, long k_ld, long k_hs,
+                      const void* v, long v_ld, long v_hs, int type, noise_stream_t stream);
+/* The values at the rows' places, rounded to `type`, into k and v [rows, kv_heads, dim] (contiguous): zero at no place, NaN at a
+ * bad one. */
+int noise_cache_read(const noise_cache_t* cache, const noise_sequences_t* seqs, void* k, void* v, int type,
+                     noise_stream_t stream);
+/* y = softmax(scale q K^T) V [rows, heads, dim] of the rows' queries q over the cached keys and values of their sequences. NaN
+ * for a row that sees a bad place; zero or left as it was (fill) for a row of no sequence. Workspace:
+ * noise_cache_attend_workspace_size(). */
+int noise_cache_attend_workspace_size(const noise_cache_t* cache, const noise_sequences_t* seqs, int heads, int window,
+                                      int sinks, size_t* bytes);
+int noise_cache_attend(const noise_cache_t* cache, const noise_sequences_t* seqs, const void* q, long q_ld, long q_hs, int type,
+                       int heads, int window, int sinks, float scale, void* y, int fill, void* workspace,
+                       size_t workspace_bytes, noise_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,8 @@ LAYOUT_ROWS, LAYOUT_TILE16, LAYOUT_WTILE = 0, 1, 2
 CE_MEMBER_MEAN, CE_NONE, CE_SUM, CE_MEAN = 0, 1, 2, 3
 HEAD_BF16, HEAD_FP32_SPLIT, HEAD_FP32 = 0, 1, 2  # noise_head_ce's weight formats (NOISE_HEAD_*)
 RESULT_BF16, RESULT_F32, RESULT_HEAD = 0, 1, 2  # noise_gemm_tile's results and tiles
+CACHE_FP4, CACHE_FP8 = 0, 1  # noise_cache_t's formats (NOISE_CACHE_*)
+ROWS_BF16, ROWS_F16, ROWS_F32 = 0, 1, 2  # row types of the serving entry points (NOISE_ROWS_*)
 TILE_256X256, TILE_256X128, TILE_128X128, TILE_64X64 = 0, 1, 2, 3
 
 # name -> argtypes in declaration order; every entry point returns int. Pointers (device buffers,
@@ -67,6 +69,11 @@ SIGNATURES = {
     'noise_adam': [P, P, P, P, L, F, F, F, F, F, P],
     'noise_adam_batch': [P, I, F, F, F, P],
     'noise_hbm_stream': [P, I, P, I, L, P],
+    'noise_sink_attention': [P, L, L, P, L, L, P, L, L, P, I, I, I, I, I, I, I, I, I, F, P, I, P],
+    'noise_cache_write': [P, P, P, L, L, P, L, L, I, P],
+    'noise_cache_read': [P, P, P, P, I, P],
+    'noise_cache_attend_workspace_size': [P, P, I, I, I, SP],
+    'noise_cache_attend': [P, P, P, L, L, I, I, I, I, F, P, I, P, S, P],
 }
 
 
@@ -173,6 +180,18 @@ def pending(*items):
         return None, 0
     arr = (Pending * len(items))(*[Pending(*it) for it in items])
     return ctypes.cast(arr, ctypes.c_void_p), len(items)
+
+
+class Cache(ctypes.Structure):
+    """noise_cache_t of include/noise_hip.h."""
+    _fields_ = [('keys', P), ('key_scales', P), ('values', P), ('value_scales', P), ('pages', L), ('page_size', I),
+                ('kv_heads', I), ('dim', I), ('format', I)]
+
+
+class Sequences(ctypes.Structure):
+    """noise_sequences_t of include/noise_hip.h."""
+    _fields_ = [('table', P), ('table_ld', L), ('table_pages', I), ('lengths', P), ('starts', P), ('sequences', I),
+                ('rows', I)]
 
 
 # Entry points whose int result is a value, not a status.

@@ -12,6 +12,7 @@
 #include "gemm.h"
 #include "probes.h"
 #include "rowops.h"
+#include "serve.h"
 
 static_assert(NOISE_QK_BF16 == QK_BF16 && NOISE_QK_F16 == QK_F16 && NOISE_QK_F16_Q_LOG2 == QK_F16_Q_LOG2 &&
                   NOISE_QK_BF16_V_BF16 == QK_BF16_V_BF16,
@@ -19,6 +20,9 @@ static_assert(NOISE_QK_BF16 == QK_BF16 && NOISE_QK_F16 == QK_F16 && NOISE_QK_F16
 static_assert(NOISE_CE_MEMBER_MEAN == CE_MEMBER_MEAN && NOISE_CE_NONE == CE_NONE && NOISE_CE_SUM == CE_SUM &&
                   NOISE_CE_MEAN == CE_MEAN,
               "reduction codes");
+static_assert(NOISE_CACHE_FP4 == CACHE_FP4 && NOISE_CACHE_FP8 == CACHE_FP8 && NOISE_ROWS_BF16 == ROWS_BF16 &&
+                  NOISE_ROWS_F16 == ROWS_F16 && NOISE_ROWS_F32 == ROWS_F32,
+              "cache formats and row types");
 
 // The moment partials of noise_attention_noalloc live in this library-owned device array: every GPU the library
 // runs on holds its own copy (16 MiB) until the process ends. In host code `scratch` only names the symbol, not a
@@ -110,6 +114,16 @@ int scratch_address(void** out) {
   }
   *out = scratch_dev[dev];
   return NOISE_OK;
+}
+
+// The C-ABI descriptions of a cache and of a call's rows; false for a null one or a page size that is no power of two.
+bool copy_cache(const noise_cache_t* src, const noise_sequences_t* seqs, Cache* c, Sequences* s) {
+  if (!src || !seqs || src->page_size <= 0 || (src->page_size & (src->page_size - 1))) return false;
+  *c = Cache{static_cast<uint8_t*>(src->keys), static_cast<uint8_t*>(src->key_scales), static_cast<uint8_t*>(src->values),
+             static_cast<uint8_t*>(src->value_scales), src->pages, __builtin_ctz(src->page_size), src->kv_heads, src->dim,
+             src->format};
+  *s = Sequences{seqs->table, seqs->table_ld, seqs->table_pages, seqs->lengths, seqs->starts, seqs->sequences, seqs->rows};
+  return true;
 }
 
 }  // namespace
@@ -673,6 +687,52 @@ int noise_adam(float* param, const float* grad, float* exp_avg, float* exp_avg_s
                float beta1, float beta2, float eps, float bc2_sqrt, noise_stream_t stream) {
   const AdamTensor t{param, grad, exp_avg, exp_avg_sq, n, step_size, bc2_sqrt};
   return adam_batch_launch(&t, 1, beta1, beta2, eps, static_cast<hipStream_t>(stream));
+}
+
+int noise_sink_attention(const void* q, long q_ld, long q_hs, const void* k, long k_ld, long k_hs, const void* v, long v_ld,
+                         long v_hs, const int* starts, int sequences, int rows, int T, int heads, int kv_heads, int dim,
+                         int type, int window, int sinks, float scale, void* y, int fill, noise_stream_t stream) {
+  const SinkArgs a{{q, q_ld, q_hs}, {k, k_ld, k_hs}, {v, v_ld, v_hs}, starts, sequences, rows, T, heads, kv_heads, dim,
+                   type, window, sinks, fill, scale, y};
+  return sink_attention_launch(a, static_cast<hipStream_t>(stream));
+}
+
+int noise_cache_write(const noise_cache_t* cache, const noise_sequences_t* seqs, const void* k, long k_ld, long k_hs,
+                      const void* v, long v_ld, long v_hs, int type, noise_stream_t stream) {
+  Cache c;
+  Sequences s;
+  if (!copy_cache(cache, seqs, &c, &s)) return NOISE_EINVAL;
+  return cache_write_launch(c, s, Heads{k, k_ld, k_hs}, Heads{v, v_ld, v_hs}, type, static_cast<hipStream_t>(stream));
+}
+
+int noise_cache_read(const noise_cache_t* cache, const noise_sequences_t* seqs, void* k, void* v, int type,
+                     noise_stream_t stream) {
+  Cache c;
+  Sequences s;
+  if (!copy_cache(cache, seqs, &c, &s)) return NOISE_EINVAL;
+  return cache_read_launch(c, s, k, v, type, static_cast<hipStream_t>(stream));
+}
+
+int noise_cache_attend_workspace_size(const noise_cache_t* cache, const noise_sequences_t* seqs, int heads, int window,
+                                      int sinks, size_t* bytes) {
+  Cache c;
+  Sequences s;
+  if (!bytes || !copy_cache(cache, seqs, &c, &s)) return NOISE_EINVAL;
+  AttendArgs a{};
+  a.heads = heads;
+  a.window = window;
+  a.sinks = sinks;
+  return cache_attend_workspace(c, s, a, bytes);
+}
+
+int noise_cache_attend(const noise_cache_t* cache, const noise_sequences_t* seqs, const void* q, long q_ld, long q_hs, int type,
+                       int heads, int window, int sinks, float scale, void* y, int fill, void* workspace,
+                       size_t workspace_bytes, noise_stream_t stream) {
+  Cache c;
+  Sequences s;
+  if (!copy_cache(cache, seqs, &c, &s)) return NOISE_EINVAL;
+  const AttendArgs a{{q, q_ld, q_hs}, type, heads, window, sinks, fill, scale, y};
+  return cache_attend_launch(c, s, a, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

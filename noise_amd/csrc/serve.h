@@ -1,0 +1,102 @@
+// Internal interface of the serving kernels (not part of the C ABI): the microscaled key / value cache and the attention of
+// prompts and of cached sequences.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+// Codes of a cache: e2m1 (two to a byte, the even channel in the low half) or e4m3. Values of the C ABI's format.
+enum : int { CACHE_FP4 = 0, CACHE_FP8 = 1 };
+// Types of rows handed in or out (values of the C ABI's type).
+enum : int { ROWS_BF16 = 0, ROWS_F16 = 1, ROWS_F32 = 2 };
+
+// keys / values [pages, kv_heads, page, dim / 2 or dim] codes; scales [pages, kv_heads, page, dim / 32] bytes: code * 2^(byte -
+// 127), 255 = NaN.
+struct Cache {
+  uint8_t *k, *ks, *v, *vs;
+  long pages;
+  int page_shift, kv_heads, dim, format;
+};
+
+// `rows` packed rows of n sequences: sequence b owns rows starts[b] .. starts[b + 1] (starts null: row b alone), its m rows at
+// the positions lengths[b] - m .. lengths[b] - 1; position p lies in page table[b * table_ld + p / page].
+struct Sequences {
+  const int* table;
+  long table_ld;
+  int table_pages;
+  const int *lengths, *starts;
+  int n, rows;
+};
+
+// 16- or 32-bit rows: head h of row r at p + r * ld + h * hs (elements).
+struct Heads {
+  const void* p;
+  long ld, hs;
+};
+
+// Whether the description of a cache and its sequences is refused.
+bool bad_cache(const Cache& c, const Sequences& s);
+int cache_write_launch(const Cache& c, const Sequences& s, const Heads& k, const Heads& v, int type, hipStream_t stream);
+int cache_read_launch(const Cache& c, const Sequences& s, void* k, void* v, int type, hipStream_t stream);
+
+struct AttendArgs {
+  Heads q;
+  int type, heads, window, sinks, fill;  // fill: rows of no sequence are set to zero (left as they were otherwise)
+  float scale;
+  void* y;  // [rows, heads, dim] of q's type
+};
+int cache_attend_launch(const Cache& c, const Sequences& s, const AttendArgs& a, void* ws, size_t ws_bytes, hipStream_t stream);
+int cache_attend_workspace(const Cache& c, const Sequences& s, const AttendArgs& a, size_t* bytes);
+
+// Attention of whole sequences: rows packed by starts (null: n sequences of T rows each).
+struct SinkArgs {
+  Heads q, k, v;
+  const int* starts;
+  int n, rows, T, heads, kv_heads, dim;
+  int type, window, sinks, fill;
+  float scale;
+  void* y;
+};
+int sink_attention_launch(const SinkArgs& a, hipStream_t stream);
+
+// ---------------------------------------------------------------- device helpers
+
+// The sequence that owns row i: the number of entries of starts[1 .. n] that are <= i, found by a wave 64 entries at a time
+// (one round of loads up to 64 sequences, two up to 4096). Rows of no sequence give n. Called by whole waves.
+__device__ __forceinline__ int find_sequence(const int* starts, int n, int i) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = n;  // the answer lies in [lo, hi]
+  while (hi - lo > 64) {
+    const int step = (hi - lo + 63) / 64;
+    const int at = lo + (lane + 1) * step;  // probe entry `at`: starts[at] <= i means the answer is >= at
+    const unsigned long long m = __ballot(at <= hi && starts[at] <= i);
+    const int k = m == ~0ull ? 64 : __builtin_ctzll(~m);
+    const int nlo = lo + k * step;
+    hi = max(nlo, min(hi, nlo + step - 1));
+    lo = nlo;
+  }
+  const int at = lo + lane + 1;
+  const unsigned long long m = __ballot(at <= hi && starts[at] <= i);
+  return lo + __builtin_popcountll(m);
+}
+
+// Row i's sequence and position; position -1 and b = -1 for a row of no sequence.
+struct Place {
+  int b;
+  long pos;
+};
+__device__ __forceinline__ Place place_of(const Sequences& s, int i) {
+  if (!s.starts) return i < s.n ? Place{i, (long)s.lengths[i] - 1} : Place{-1, -1};
+  const int b = __builtin_amdgcn_readfirstlane(find_sequence(s.starts, s.n, i));
+  if (b >= s.n) return Place{-1, -1};
+  const int s0 = s.starts[b], s1 = s.starts[b + 1];
+  if (i < s0 || i >= s1) return Place{-1, -1};
+  return Place{b, (long)s.lengths[b] - s1 + i};
+}
+// The slot (page * page size + token) of a position, or -1 where the table names no page of the cache for it.
+__device__ __forceinline__ long slot_of(const Cache& c, const Sequences& s, int b, long pos) {
+  const long pg = pos >> c.page_shift;
+  if (pos < 0 || pg >= s.table_pages) return -1;
+  const int id = s.table[b * s.table_ld + pg];
+  if (id < 0 || id >= c.pages) return -1;
+  return ((long)id << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+}

@@ -4,6 +4,8 @@ Each op validates shapes and dtypes on the host, allocates its outputs and works
 enqueues the HIP kernels on torch's current stream. Inputs must already be CUDA tensors: there is no
 CPU path.
 """
+import math
+
 import torch
 
 from . import _lib
@@ -112,3 +114,111 @@ def lowrank_mlp(x, w_fc, w_proj, a_fc, b_fc, a_proj, b_proj, sign, T=None, pair_
 
 def mlp_workspace_bytes(members, T, d=512, f=2048):
     return _lib.size_query('noise_lowrank_mlp_workspace_size', members, T, d, f)
+
+
+ROW_TYPES = {torch.bfloat16: _lib.ROWS_BF16, torch.float16: _lib.ROWS_F16, torch.float32: _lib.ROWS_F32}
+NO_WINDOW = 2 ** 31 - 1
+
+
+def no_grad_rows(*tensors):
+    """The serving operators are forward-only: refuse a tensor whose gradient a caller would expect."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError('the serving operators have no backward pass: call them under torch.no_grad() or detach the inputs')
+
+
+def one_device(*tensors):
+    """The CUDA device that all of them are on."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t.device.type != 'cuda':
+            raise ValueError('the operands must be CUDA tensors (no CPU path)')
+        if t.device != dev:
+            raise ValueError(f'the operands are on different devices ({dev} and {t.device})')
+    return dev
+
+
+def heads_rows(t):
+    """(tensor to keep alive, pointer, row stride, head stride) of rows [n, heads, dim] as the kernels read them: in place
+    where the channels are contiguous and rows and heads start at 16-byte addresses, else from a contiguous copy."""
+    unit = 16 // t.element_size()
+    n, heads, dim = t.shape
+    # (the stride of a dimension of one entry means nothing)
+    ld, hs = t.stride(0) if n > 1 else 0, t.stride(1) if heads > 1 else 0
+    if t.stride(2) != 1 or ld % unit or hs % unit or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        ld, hs = heads * dim, dim
+    return t, t.data_ptr(), ld, hs
+
+
+def mask_args(window, sinks, scale, dim):
+    """(window, sinks, scale) as the entry points take them."""
+    window = NO_WINDOW if window is None else int(window)
+    sinks = int(sinks)
+    if window < 0 or sinks < 0:
+        raise ValueError('window (None for no window) and sinks must be >= 0')
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0 <= scale < math.inf:
+        raise ValueError('scale must be finite and >= 0')
+    return min(window, NO_WINDOW), min(sinks, NO_WINDOW), scale
+
+
+def sequence_starts(starts, dev):
+    """Checks the packed rows' starts and returns the number of sequences."""
+    if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() < 1 or not starts.is_contiguous():
+        raise ValueError('starts must be a contiguous int32 vector of sequences + 1 entries')
+    one_device(torch.empty(0, device=dev), starts)
+    return starts.numel() - 1
+
+
+def output_rows(out, like, dev):
+    """The output [n, heads, dim] and whether rows of no sequence are to be zeroed (not in a tensor the caller gave)."""
+    if out is None:
+        return torch.empty(like.shape, device=dev, dtype=like.dtype), 1
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f'out must be a contiguous {like.dtype} tensor of shape {tuple(like.shape)} beside q, 16-byte aligned')
+    no_grad_rows(out)
+    return out, 0
+
+
+def sink_attention(q, k, v, starts=None, window=None, sinks=0, scale=None, out=None):
+    """Causal attention of whole sequences with a left window and first tokens that stay visible: a query at position s sees
+    the keys j <= s with s - j <= window (None: all of them) or j < sinks.
+
+    q [n, heads, dim], k and v [n, kv_heads, dim] are packed rows of sequences of any lengths, sequence b owning rows
+    starts[b] .. starts[b + 1] (int32 on the GPU, nondecreasing); or, without starts, [batch, T, heads, dim] and [batch, T,
+    kv_heads, dim]. bf16 or fp16, dim 64 or 128, heads a multiple of kv_heads; any strides (read in place when the channels
+    are contiguous and rows and heads are 16-byte aligned). scale defaults to dim ** -0.5. Returns q's shape and type. A
+    row that sees no key is zero; what a row does not see takes no part in it, infinities and NaN included. Rows of no
+    sequence come back zero, or, in a given `out` (which must not overlap the inputs), stay as they were. Forward only."""
+    no_grad_rows(q, k, v)
+    dev = one_device(q, k, v)
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f'q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}')
+    nd = 4 if starts is None else 3
+    if q.dim() != nd or k.shape != v.shape or k.dim() != nd or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+        raise ValueError('q must be [n, heads, dim] and k, v [n, kv_heads, dim] with starts, [batch, T, ...] without; got '
+                         f'{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
+    heads, dim = q.shape[-2:]
+    kv = k.shape[-2]
+    if dim not in (64, 128) or kv == 0 or heads == 0 or heads % kv or heads > 1024:
+        raise ValueError(f'dim must be 64 or 128 and heads (at most 1024) a multiple of kv_heads: got {heads} x {dim} on {kv}')
+    window, sinks, scale = mask_args(window, sinks, scale, dim)
+    y, fill = output_rows(out, q, dev)
+    T = 0
+    if starts is None:
+        n, T = q.shape[:2]
+        q, k, v = q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1)
+    else:
+        n = sequence_starts(starts, dev)
+    rows = q.shape[0]
+    if rows == 0:
+        return y
+    if n == 0:  # no sequence at all: every row is behind the last one
+        return y.zero_() if fill else y
+    q, qp, ql, qh = heads_rows(q)
+    k, kp, kl, kh = heads_rows(k)
+    v, vp, vl, vh = heads_rows(v)
+    with torch.cuda.device(dev):
+        _lib.call('noise_sink_attention', qp, ql, qh, kp, kl, kh, vp, vl, vh, _ptr(starts), n, rows, T, heads, kv, dim,
+                  ROW_TYPES[q.dtype], window, sinks, scale, y.data_ptr(), fill, _stream())
+    return y
