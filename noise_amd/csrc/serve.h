@@ -34,6 +34,9 @@ struct Heads {
 };
 
 // Whether the description of a cache and its sequences is refused.
+inline bool bad_heads(const Heads& h) {
+  return !h.p || ((uintptr_t)h.p & 15) || h.ld < 0 || h.hs < 0 || h.ld % 8 || h.hs % 8;
+}
 bool bad_cache(const Cache& c, const Sequences& s);
 int cache_write_launch(const Cache& c, const Sequences& s, const Heads& k, const Heads& v, int type, hipStream_t stream);
 int cache_read_launch(const Cache& c, const Sequences& s, void* k, void* v, int type, hipStream_t stream);

@@ -308,6 +308,22 @@ def test_rows_at_no_place_and_at_bad_ones():
     assert not cache.keys.any()
 
 
+def test_rows_before_and_past_the_table():
+    """A sequence longer than its table: the rows at positions that the table names are attended to, the others are NaN."""
+    f = Filled([128], 2, 64, 'fp4', 16, seed=13)
+    q = rows(torch.Generator().manual_seed(14), 40, 4, 64, BF16)
+    pos = torch.arange(95, 135)
+    y, terms = plain.attend(q, *f.held[0], pos.clamp(max=127), 50, 3)
+    got = f.cache.attend(q.to(DEV), f.table, i32([135]), i32([0, 40]), window=50, sinks=3).cpu()
+    assert torch.isnan(got[pos > 127]).all()
+    ok = pos <= 127
+    check(got[ok], y[ok], tuple(t[ok] for t in terms), BF16, P_CACHE)
+    x = torch.ones(40, 2, 64, device=DEV, dtype=BF16)
+    f.cache.write(x, x, f.table, i32([135]), i32([0, 40]))
+    k, _ = f.cache.read(f.table, i32([135]), i32([0, 40]), rows=40)
+    assert (k[:33] == 1).all() and torch.isnan(k[33:]).all()
+
+
 def test_nothing_is_written_or_read_for_no_rows():
     cache = KVCache.zeros(2, 1, 64, 16, 'fp4')
     x = torch.ones(3, 1, 64, device=DEV, dtype=BF16)
@@ -338,7 +354,7 @@ ATTEND = [
     ([700, 800, 900], None, 3, 3, 128, 'fp4', 64, BF16, 1, 300),
     ([1300], None, 64, 1, 64, 'fp4', 64, F16, None, 0),
 ]
-P_CACHE = None  # type the probabilities are rounded to in front of the values
+P_CACHE = BF16  # bf16 queries' probabilities are rounded to bf16 in front of the values; fp16's are two bf16 terms
 
 
 def attend_reference(f, q, new, window, sinks, scale=None):
@@ -359,7 +375,7 @@ def test_attention_over_the_cache(case):
     y, terms = attend_reference(f, q, m, window, sinks)
     st = i32(starts_of(m)) if new else None
     got = f.cache.attend(q.to(DEV), f.table, f.lengths, st, window=window, sinks=sinks)
-    check(got, y, terms, dtype, P_CACHE)
+    check(got, y, terms, dtype, P_CACHE if dtype == BF16 else None)
 
 
 def test_cache_scale_and_large_scores():
