@@ -27,11 +27,8 @@ namespace {
 
 typedef _Float16 f16;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4_t;
 
 constexpr int RT = 16;         // rows of a tile
-constexpr float LAZY = 8.f;    // the maximum moves only beyond 2^8 of headroom
 
 template <int DIM, int FMT>
 struct Geo {
@@ -61,13 +58,6 @@ __device__ __forceinline__ u32x4 bf16_of(const unsigned* w, float scale) {
     r[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], scale, true));
   }
   return r;
-}
-
-// 16-byte chunk of V row R (16 dims' halves of 8): XOR-swizzled so that the rows of a transposing read (8 g + 4 h + t, four t of
-// two lane groups g in a cycle of 32 lanes) cover the banks once.
-template <int DIM>
-__device__ __forceinline__ int vswz(int R) {
-  return DIM == 64 ? 2 * (((R >> 1) & 1) | ((((R >> 3) ^ R) & 1) << 1)) : 2 * ((R & 3) | (((R >> 3) & 1) << 2));
 }
 
 // One sequence's share of a call, as the kernels cut it.
@@ -118,12 +108,6 @@ __device__ __forceinline__ Cut cut_of(const Sequences& s, const Plan& p, int pag
     c.blocks = range_of(last + 1 - span, last, window, sinks, p.block_shift).blocks + (c.tiles > 1);
   }
   return c;
-}
-
-// x of lane k in a scalar register (a lane shuffle's result counts as a lane's own, and so would all that follows from it)
-__device__ __forceinline__ int uniform(int x, int k = 0) { return __builtin_amdgcn_readlane(x, k); }
-__device__ __forceinline__ long uniform(long x, int k = 0) {
-  return (long)((unsigned long long)(unsigned)uniform((int)(x >> 32), k) << 32 | (unsigned)uniform((int)x, k));
 }
 
 struct Work {
@@ -178,15 +162,6 @@ __device__ Work find_work(const Sequences& s, const Plan& p, int page_shift, int
   return w;
 }
 
-// Zeroes the rows of no sequence: in front of the first one and behind the last.
-template <int DIM>
-__device__ void fill_rows(const Sequences& s, void* y, int heads, int nth, int part, int parts) {
-  const int lo = min(max(s.starts[0], 0), s.rows), hi = min(max(s.starts[s.n], lo), s.rows);
-  const long units = (long)heads * DIM / 8, head = lo * units, all = head + (s.rows - hi) * units;
-  for (long i = (long)part * nth + threadIdx.x; i < all; i += (long)parts * nth)
-    static_cast<uint4*>(y)[i < head ? i : hi * units + i - head] = make_uint4(0, 0, 0, 0);
-}
-
 struct Args {
   Cache c;
   Sequences s;
@@ -211,7 +186,7 @@ __global__ void __launch_bounds__(64 * NW, 3) attend_kernel(Args g) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, grp = lane >> 4;
   if ((int)blockIdx.x >= g.items) {
-    fill_rows<DIM>(s, g.a.y, g.a.heads, 64 * NW, blockIdx.x - g.items, g.fills);
+    fill_rows(s.starts, s.n, s.rows, g.a.y, g.a.heads * DIM, 64 * NW, blockIdx.x - g.items, g.fills);
     return;
   }
   const int kh = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads;

@@ -103,3 +103,28 @@ __device__ __forceinline__ long slot_of(const Cache& c, const Sequences& s, int 
   if (id < 0 || id >= c.pages) return -1;
   return ((long)id << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
 }
+
+// x of lane k in a scalar register (a lane shuffle's result counts as a lane's own, and so would all that follows from it)
+__device__ __forceinline__ int uniform(int x, int k = 0) { return __builtin_amdgcn_readlane(x, k); }
+__device__ __forceinline__ long uniform(long x, int k = 0) {
+  return (long)((unsigned long long)(unsigned)uniform((int)(x >> 32), k) << 32 | (unsigned)uniform((int)x, k));
+}
+
+// Zeroes the rows of no sequence, in front of the first one and behind the last: workgroup `part` of `parts` of nth threads.
+__device__ __forceinline__ void fill_rows(const int* starts, int n, int rows, void* y, int width, int nth, int part, int parts) {
+  const int lo = min(max(starts[0], 0), rows), hi = min(max(starts[n], lo), rows);
+  const long units = width / 8, head = lo * units, all = head + (rows - hi) * units;
+  for (long i = (long)part * nth + threadIdx.x; i < all; i += (long)parts * nth)
+    static_cast<uint4*>(y)[i < head ? i : hi * units + i - head] = make_uint4(0, 0, 0, 0);
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4_t;
+constexpr float LAZY = 8.f;  // a running maximum moves only beyond 2^8 of headroom
+
+// 16-byte chunk of V row R (16 dims' halves of 8): XOR-swizzled so that the rows of a transposing read (8 g + 4 h + t, four t of
+// two lane groups g in a cycle of 32 lanes) cover the banks once.
+template <int DIM>
+__device__ __forceinline__ int vswz(int R) {
+  return DIM == 64 ? 2 * (((R >> 1) & 1) | ((((R >> 3) ^ R) & 1) << 1)) : 2 * ((R & 3) | (((R >> 3) & 1) << 2));
+}

@@ -1,6 +1,19 @@
-// Attention of whole prompts and of rows over the key / value cache: a query at position s sees key j when 0 <= j <= s and
-// (s - j <= window or j < sinks). One wave per row and head: 64 keys at a time, a lane a key for the scores, a lane a channel
-// for the values; the running maximum and sum of the softmax in fp32.
+// Causal attention of whole sequences with a left window and sinks: a query at position s sees key j <= s when s - j <= window or
+// j < sinks. Sequences of any lengths are packed in one call, heads may be grouped over fewer kv heads.
+//
+// Bound: for dim 64 the softmax's vector work (an exponential, a fused multiply-add, half a maximum and half a conversion a score,
+// beside 4 x 64 flop on the matrix cores), for dim 128 the matrix cores.
+//
+// One workgroup takes 64 QB queries of one sequence and head, a wave 16 QB of them; key blocks of 64 go through a double-buffered
+// LDS ring by direct global -> LDS loads, block j + 1 landing while block j is computed.
+//   S^T = K Q^T (A = K rows, B = Q rows): a lane holds 16 scores of query lane % 16. K rows are interleaved at load time so that
+//   the scores' layout is the B operand of O^T += V^T P^T: P never leaves registers. V stays row-major [key][channel] and
+//   its A fragments come from transposing LDS reads.
+//   Softmax in fp32 with a lazy running maximum; P is rounded once to the operands' type, and its row sums are taken of the rounded
+//   values on the matrix cores (an all-ones operand), so that the rounding cancels in part.
+// Blocks between the sinks and the window are skipped, and a wave skips the blocks none of its queries sees. Blocks seen in part are
+// masked; should such a block hold infinities or NaN among its values, it is multiplied row by row with what the row does not
+// see taken out, since 0 x NaN is not 0.
 #include <type_traits>
 
 #include "common.h"
@@ -9,101 +22,383 @@
 namespace {
 
 typedef _Float16 f16;
-constexpr int WAVES = 4, NTH = 64 * WAVES;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float load1(const void* p, long at, int type) {
-  return type == ROWS_F16 ? (float)static_cast<const f16*>(p)[at] : (float)static_cast<const bf16*>(p)[at];
-}
-__device__ __forceinline__ float wave_max(float x) {
-  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-  return x;
-}
-__device__ __forceinline__ float wave_add(float x) {
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o, 64);
-  return x;
-}
+constexpr int BKV = 64, NWAVE = 4, NTH = 64 * NWAVE;
+constexpr int KB = BKV / 16, KC = BKV / 32;  // 16-key tiles of a block, 32-key steps of P V
 
-// key(j, d), value(j, d): channel d of key j
-template <class K, class V>
-__device__ void attend_row(const float* q, int dim, long pos, int window, int sinks, float scale, K key, V value, float (&y)[2]) {
-  const int lane = threadIdx.x & 63;
-  const long lo = max(0l, pos - window), first = min((long)sinks, lo), n = first + pos - lo + 1;
-  float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
-  for (long t0 = 0; t0 < n; t0 += 64) {
-    const long t = t0 + lane;
-    float s = -INFINITY;
-    if (t < n) {
-      const long j = t < first ? t : lo + t - first;
-      float d = 0.f;
-      for (int c = 0; c < dim; ++c) d = fmaf(q[c], key(j, c), d);
-      s = d * scale;
-    }
-    // a NaN score makes the maximum NaN, and so the row
-    const float top = wave_max(s);
-    const float mn = __any(s != s) ? __uint_as_float(0x7fc00000u) : fmaxf(m, top);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __expf(m - base), p = __expf(s - base);
-    m = mn;
-    l = l * alpha + wave_add(p);
-    o[0] *= alpha, o[1] *= alpha;
-    const int cnt = (int)min(64l, n - t0);
-    for (int k = 0; k < cnt; ++k) {
-      const float pk = __shfl(p, k, 64);
-      const long tk = t0 + k, j = tk < first ? tk : lo + tk - first;
-      for (int c = 0; c < dim / 64; ++c) o[c] = fmaf(pk, value(j, lane + 64 * c), o[c]);
-    }
-  }
-  for (int c = 0; c < 2; ++c) y[c] = l == 0.f ? 0.f : o[c] / l;
-}
-
-template <class T>
-__device__ void put(T* y, int dim, const float (&v)[2]) {
-  for (int c = 0; c < dim / 64; ++c) y[(threadIdx.x & 63) + 64 * c] = (T)v[c];
-}
-__device__ void put_row(void* y, long at, int type, int dim, const float (&v)[2]) {
-  if (type == ROWS_F16)
-    put(static_cast<f16*>(y) + at, dim, v);
+template <bool F16>
+struct Elem {
+  using T = typename std::conditional<F16, f16, bf16>::type;
+  typedef T x8 __attribute__((ext_vector_type(8)));
+  typedef T x4 __attribute__((ext_vector_type(4)));
+};
+template <bool F16, class X>
+__device__ __forceinline__ f32x4 mfma(const X& a, const X& b, const f32x4& c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   else
-    put(static_cast<bf16*>(y) + at, dim, v);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-__global__ void __launch_bounds__(NTH) sink_kernel(SinkArgs a) {
-  __shared__ float sq[WAVES][128];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const long i = (long)blockIdx.x * WAVES + wave;
-  if (i >= (long)a.rows * a.heads) return;
-  const int row = (int)(i / a.heads), h = (int)(i % a.heads), kh = h / (a.heads / a.kv_heads);
-  int s0 = 0;
-  bool mine = true;
+// Key of LDS row R of a K block.
+__device__ __forceinline__ int key_of_row(int R) {
+  const int kb = R >> 4, r = R & 15;
+  return 32 * (kb >> 1) + 8 * (r >> 2) + 4 * (kb & 1) + (r & 3);
+}
+// 16-byte chunk swizzle of LDS row R of a K block: the 16 rows of a fragment's read cover the banks once.
+template <int DIM>
+__device__ __forceinline__ int kswz(int R) {
+  return DIM == 64 ? R & 7 : R & 15;
+}
+
+struct Args {
+  SinkArgs a;
+  float c2;          // scale in base-2 units
+  int items, fills;  // workgroups of tiles, workgroups that zero rows
+};
+
+struct Tile {
+  int s0, m, q0, h;  // first row and rows of the sequence, first query, head
+  bool found;
+};
+
+// The tile of workgroup `id`. Workgroups reach the 8 XCDs in turn. Where heads divide by 8, XCD x takes the heads x heads / 8 .. of
+// every sequence, so all XCDs have the same work and the tiles that share keys run on one XCD's L2; otherwise XCD x takes a
+// contiguous range of all tiles in (sequence, head, tile) order. Later tiles, which see more keys, come first.
+template <int BQ>
+__device__ Tile find_tile(const SinkArgs& a, int id) {
+  const int lane = threadIdx.x & 63, x = id & 7, j = id >> 3;
+  const bool even = a.heads % 8 == 0;
+  const int per = even ? a.heads / 8 : a.heads;  // heads that an index runs over
+  Tile t{};
+  auto rows_of = [&](int b, int& s0) {
+    s0 = 0;
+    if (b >= a.n) return 0;
+    if (!a.starts) {
+      s0 = b * a.T;
+      return a.T;
+    }
+    s0 = min(max(a.starts[b], 0), a.rows);
+    return min(max(a.starts[b + 1], s0), a.rows) - s0;
+  };
+  long at = j;
+  if (!even) {
+    long total = 0;
+    int s0;
+    if (a.starts) {
+      for (int b0 = 0; b0 < a.n; b0 += 64) total += (rows_of(b0 + lane, s0) + BQ - 1) / BQ;
+      for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
+      total = uniform(total);
+    } else {
+      total = (long)a.n * ((a.T + BQ - 1) / BQ);
+    }
+    total *= per;
+    const long q = total / 8, r = total % 8;
+    if (j >= q + (x < r)) return t;
+    at = x * q + min((long)x, r) + j;
+  }
+  auto take = [&](int s0, int m, long i) {
+    const int tiles = (m + BQ - 1) / BQ, hh = (int)(i / tiles);
+    t.found = true;
+    t.s0 = s0;
+    t.m = m;
+    t.q0 = (tiles - 1 - (int)(i % tiles)) * BQ;
+    t.h = even ? x * per + hh : hh;
+  };
   if (!a.starts) {
-    s0 = row / a.T * a.T;
-  } else {
-    const int b = __builtin_amdgcn_readfirstlane(find_sequence(a.starts, a.n, row));
-    mine = b < a.n && a.starts[b] >= 0 && a.starts[b] <= row && row < a.starts[b + 1];
-    if (mine) s0 = a.starts[b];
+    const long each = (long)((a.T + BQ - 1) / BQ) * per;
+    const long b = at / each;
+    if (b < a.n) take((int)b * a.T, a.T, at % each);
+    return t;
   }
-  if (!mine && !a.fill) return;
-  float y[2] = {0.f, 0.f};
-  if (mine) {
-    for (int d = lane; d < a.dim; d += 64) sq[wave][d] = load1(a.q.p, row * a.q.ld + h * a.q.hs + d, a.type);
-    __builtin_amdgcn_wave_barrier();
-    attend_row(sq[wave], a.dim, row - s0, a.window, a.sinks, a.scale,
-               [&](long j, int d) { return load1(a.k.p, (s0 + j) * a.k.ld + kh * a.k.hs + d, a.type); },
-               [&](long j, int d) { return load1(a.v.p, (s0 + j) * a.v.ld + kh * a.v.hs + d, a.type); }, y);
+  long base = 0;
+  for (int b0 = 0; b0 < a.n; b0 += 64) {
+    int s0;
+    const int m = rows_of(b0 + lane, s0);
+    const long mine = (long)((m + BQ - 1) / BQ) * per;
+    long upto = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+      const long u = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += u;
+    }
+    const unsigned long long hits = __ballot(at < base + upto);
+    if (hits) {
+      const int k = __builtin_ctzll(hits);
+      take(uniform(s0, k), uniform(m, k), at - base - uniform(upto - mine, k));
+      return t;
+    }
+    base += uniform(upto, 63);
   }
-  put_row(a.y, ((long)row * a.heads + h) * a.dim, a.type, a.dim, y);
+  return t;
+}
+
+template <int DIM, bool F16, int QB>
+__global__ void __launch_bounds__(NTH, DIM == 64 ? 3 : 2) sink_kernel(Args g) {
+  using E = Elem<F16>;
+  using T = typename E::T;
+  using x8 = typename E::x8;
+  using x4 = typename E::x4;
+  constexpr int BQ = 64 * QB, QS = DIM / 32, DT = DIM / 16;
+  constexpr int ROWB = 2 * DIM, CH = DIM / 8;          // bytes and 16-byte chunks of a row
+  constexpr int DH = BKV * ROWB / 1024 / NWAVE;        // load instructions of 1 KiB per wave, block and operand
+  constexpr int RPI = 1024 / ROWB;                     // rows of one
+  __shared__ __attribute__((aligned(1024))) char sk[2][BKV * ROWB];
+  __shared__ __attribute__((aligned(1024))) char sv[2][BKV * ROWB];
+  const SinkArgs& a = g.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = lane >> 4, r16 = lane & 15;
+  if ((int)blockIdx.x >= g.items) {
+    fill_rows(a.starts, a.n, a.rows, a.y, a.heads * DIM, NTH, blockIdx.x - g.items, g.fills);
+    return;
+  }
+  const Tile w = find_tile<BQ>(a, blockIdx.x);
+  if (!w.found) return;
+  const int kh = w.h / (a.heads / a.kv_heads), last = w.m - 1;
+  const T* qp = static_cast<const T*>(a.q.p) + (long)w.s0 * a.q.ld + w.h * a.q.hs;
+  const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(a.k.p) + (long)w.s0 * a.k.ld + kh * a.k.hs);
+  const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(a.v.p) + (long)w.s0 * a.v.ld + kh * a.v.hs);
+
+  // this wave's queries qw .. qe; rows past the sequence repeat its last one and are not stored
+  const int qw = w.q0 + 16 * QB * wave, qe = min(qw + 16 * QB - 1, last);
+  x8 qf[QB][QS];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+    for (int i = 0; i < QS; ++i)
+      qf[qb][i] = *reinterpret_cast<const x8*>(qp + (long)min(qw + 16 * qb + r16, last) * a.q.ld + 32 * i + 8 * grp);
+
+  // the workgroup's blocks: the sinks', then from the window's first key to the last query
+  const int qlast = min(w.q0 + BQ - 1, last), first = w.q0 > a.window ? w.q0 - a.window : 0;
+  const int lo = first / BKV, sink = min((min(a.sinks, first) + BKV - 1) / BKV, lo), blocks = sink + qlast / BKV - lo + 1;
+  auto block_key = [&](int i) { return (i < sink ? i : lo + i - sink) * BKV; };
+
+  // Loads of block i into ring slot buf. Instruction d fills LDS rows RPI d ..; lane L -> row RPI d + L / CH, chunk L % CH.
+  const int lrow = lane / CH, lchunk = lane % CH;
+  unsigned koffs[DH], voffs[DH];
+#pragma unroll
+  for (int q = 0; q < DH; ++q) {
+    const int R = RPI * (DH * wave + q) + lrow;
+    koffs[q] = 2u * (unsigned)(key_of_row(R) * (int)a.k.ld + 8 * (lchunk ^ kswz<DIM>(R)));
+    voffs[q] = 2u * (unsigned)(R * (int)a.v.ld + 8 * (lchunk ^ vswz<DIM>(R)));
+  }
+  auto issue = [&](int i, int buf) {
+    const int j0 = block_key(i);
+    const char *k0 = kp + 2l * j0 * a.k.ld, *v0 = vp + 2l * j0 * a.v.ld;
+    const char *kd = sk[buf] + DH * wave * 1024, *vd = sv[buf] + DH * wave * 1024;
+    if (j0 + BKV - 1 <= last) {
+#pragma unroll
+      for (int q = 0; q < DH; ++q) dma_x4_s(k0, koffs[q], kd + 1024 * q);
+#pragma unroll
+      for (int q = 0; q < DH; ++q) dma_x4_s(v0, voffs[q], vd + 1024 * q);
+    } else {  // rows past the sequence repeat its last one (no query sees them)
+#pragma unroll
+      for (int q = 0; q < DH; ++q) {
+        const int R = RPI * (DH * wave + q) + lrow;
+        dma_x4_s(k0, 2u * (unsigned)(min(key_of_row(R), last - j0) * (int)a.k.ld + 8 * (lchunk ^ kswz<DIM>(R))), kd + 1024 * q);
+        dma_x4_s(v0, 2u * (unsigned)(min(R, last - j0) * (int)a.v.ld + 8 * (lchunk ^ vswz<DIM>(R))), vd + 1024 * q);
+      }
+    }
+  };
+
+  float mref[QB];
+  f32x4 o[QB][DT], osum[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    mref[qb] = -INFINITY;
+    osum[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[qb][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const x8 ones = {(T)1.f, (T)1.f, (T)1.f, (T)1.f, (T)1.f, (T)1.f, (T)1.f, (T)1.f};
+  // fragment i of K tile kb: row 16 kb + r16, chunk 4 i + grp; of V: key 8 grp + t (+ 32 c + 4 x), chunk pair d
+  const int kro = r16 * ROWB + 16 * (grp ^ kswz<DIM>(r16));
+  const int vrr = 8 * grp + (r16 >> 2);
+  const int vro = vrr * ROWB + 16 * (((lane & 3) >> 1) ^ vswz<DIM>(vrr)) + 8 * (lane & 1);
+
+  auto block = [&](int i, auto bufc) {
+    constexpr int buf = decltype(bufc)::value;
+    if (i + 1 < blocks) issue(i + 1, buf ^ 1);
+    const int j0 = block_key(i);
+    const char *kt = sk[buf], *vt = sv[buf];
+    // blocks that this wave's queries see in part, or not at all
+    const bool causal = j0 + BKV - 1 > qw, left = qe - j0 > a.window && j0 + BKV > a.sinks;
+    const bool none = j0 > qe || (qw - (j0 + BKV - 1) > a.window && j0 >= a.sinks);
+    if (!none) {
+      f32x4 s[QB][KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        x8 kf[QS];
+#pragma unroll
+        for (int q = 0; q < QS; ++q) kf[q] = *reinterpret_cast<const x8*>(kt + (kro ^ (64 * q)) + 16 * kb * ROWB);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          s[qb][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < QS; ++q) s[qb][kb] = mfma<F16>(kf[q], qf[qb][q], s[qb][kb]);
+        }
+      }
+      if (causal | left) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          const int q = qw + 16 * qb + r16;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = j0 + 32 * (kb >> 1) + 8 * grp + 4 * (kb & 1) + e;
+              const bool see = (j <= q) & ((q - j <= a.window) | (j < a.sinks));
+              s[qb][kb][e] = see ? s[qb][kb][e] : -INFINITY;
+            }
+        }
+      }
+      x8 pf[QB][KC];
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        float mx = fmaxf(s[qb][0][0], s[qb][0][1]);
+#pragma unroll
+        for (int x = 2; x < 4 * KB; x += 2) mx = fmaxf(mx, fmaxf(s[qb][x / 4][x % 4], s[qb][x / 4][x % 4 + 1]));
+        mx = max_rows4(mx);
+        const bool move = mx * g.c2 > mref[qb] * g.c2 + LAZY;
+        if (__any(move)) {
+          const float mnew = move ? mx : mref[qb];
+          const float alpha = move ? __builtin_amdgcn_exp2f((mref[qb] - mnew) * g.c2) : 1.f;
+          mref[qb] = mnew;
+          osum[qb] *= alpha;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[qb][d] *= alpha;
+        }
+        const float mc = mref[qb] == -INFINITY ? 0.f : mref[qb] * g.c2;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            pf[qb][c][x] = (T)__builtin_amdgcn_exp2f(fmaf(s[qb][2 * c + (x >> 2)][x & 3], g.c2, -mc));
+      }
+      auto vfrag = [&](int c, int d) {
+        const char* p = vt + (vro ^ (32 * d)) + 32 * c * ROWB;
+        const x4 l = __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
+        const x4 h = __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(p + 4 * ROWB)));
+        return x8{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+      };
+      bool odd = false;
+      if (causal | left) {
+        constexpr unsigned EXP = F16 ? 0x7c00u : 0x7f80u;
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const u32x4 v = __builtin_bit_cast(u32x4, vfrag(c, d));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= ((v[e] & EXP) == EXP) | ((v[e] & EXP << 16) == EXP << 16);
+          }
+      }
+      if (!__any(odd)) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const x8 vf = vfrag(c, d);
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) o[qb][d] = mfma<F16>(vf, pf[qb][c], o[qb][d]);
+          }
+      } else {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+#pragma unroll 1
+          for (int row = 0; row < 16; ++row) {
+            const int q = qw + 16 * qb + row;
+            int k0 = j0 + 8 * grp;
+            asm volatile("" : "+v"(k0));
+            u32x4 keep[KC];
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                unsigned mk[2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  const int j = k0 + 32 * c + 2 * x + y;
+                  mk[y] = (j <= q) & ((q - j <= a.window) | (j < a.sinks)) ? 0xffffu : 0u;
+                }
+                keep[c][x] = mk[0] | mk[1] << 16;
+              }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+              f32x4 add = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int c = 0; c < KC; ++c)
+                add = mfma<F16>(__builtin_bit_cast(x8, __builtin_bit_cast(u32x4, vfrag(c, d)) & keep[c]), pf[qb][c], add);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[qb][d][e] = r16 == row ? o[qb][d][e] + add[e] : o[qb][d][e];
+            }
+          }
+      }
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) osum[qb] = mfma<F16>(ones, pf[qb][c], osum[qb]);
+    }
+    // block i + 1 has landed for this wave, and the barrier makes every wave's part of it visible and retires slot buf
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  };
+
+  issue(0, 0);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  for (int i = 0; i < blocks; i += 2) {
+    block(i, std::integral_constant<int, 0>{});
+    if (i + 1 < blocks) block(i + 1, std::integral_constant<int, 1>{});
+  }
+
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const int q = qw + 16 * qb + r16;
+    if (q > last) continue;
+    const float inv = 1.f / osum[qb][0];
+    T* y = static_cast<T*>(a.y) + ((long)(w.s0 + q) * a.heads + w.h) * DIM + 4 * grp;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      *reinterpret_cast<x4*>(y + 16 * d) =
+          x4{(T)(o[qb][d][0] * inv), (T)(o[qb][d][1] * inv), (T)(o[qb][d][2] * inv), (T)(o[qb][d][3] * inv)};
+  }
 }
 
 }  // namespace
 
 int sink_attention_launch(const SinkArgs& a, hipStream_t stream) {
-  if (bad_heads(a.q) || bad_heads(a.k) || bad_heads(a.v) || !a.y || ((uintptr_t)a.y & 15) || (a.type != ROWS_BF16 && a.type != ROWS_F16) || (a.dim != 64 && a.dim != 128) ||
-      a.heads <= 0 || a.heads > 1024 || a.kv_heads <= 0 || a.heads % a.kv_heads || a.window < 0 || a.sinks < 0 ||
-      !(a.scale >= 0.f) || a.n <= 0 || a.rows <= 0 || (!a.starts && (a.T <= 0 || (long)a.n * a.T != a.rows)))
+  if (bad_heads(a.q) || bad_heads(a.k) || bad_heads(a.v) || !a.y || ((uintptr_t)a.y & 15) ||
+      (a.type != ROWS_BF16 && a.type != ROWS_F16) || (a.dim != 64 && a.dim != 128) || a.heads <= 0 || a.heads > 1024 ||
+      a.kv_heads <= 0 || a.heads % a.kv_heads || a.window < 0 || a.sinks < 0 || !(a.scale >= 0.f) || a.scale > 3.4e38f ||
+      a.n <= 0 || a.rows <= 0 || (!a.starts && (a.T <= 0 || (long)a.n * a.T != a.rows)))
     return NOISE_EINVAL;
-  const long waves = (long)a.rows * a.heads;
-  if (waves > 0x7fffffffL) return NOISE_ENOTSUP;
-  hipLaunchKernelGGL(sink_kernel, dim3((unsigned)((waves + WAVES - 1) / WAVES)), dim3(NTH), 0, stream, a);
+  // (byte offsets inside a 64-key block are 32-bit)
+  if (a.k.ld > (1 << 24) || a.v.ld > (1 << 24)) return NOISE_ENOTSUP;
+  // tiles: of queries, at most one begun by every sequence beside the full ones; the GPU counts them
+  auto groups = [&](int bq) {
+    const long tiles = a.starts ? a.rows / bq + (a.n < a.rows ? a.n : a.rows) : (long)a.n * ((a.T + bq - 1) / bq);
+    return a.heads % 8 == 0 ? tiles * a.heads : (tiles * a.heads + 7) / 8 * 8;
+  };
+  const bool narrow = groups(128) <= 2 * num_cus();
+  const long items = groups(narrow ? 64 : 128);
+  Args g{a, 0.f, (int)items, a.fill && a.starts ? 32 : 0};
+  if (items + g.fills > 0x7fffffffL) return NOISE_ENOTSUP;
+  // (a scale of 0 is the smallest normal number: every seen key weighs the same, and a masked score stays -infinity)
+  const float c2 = a.scale * 1.4426950408889634f;
+  g.c2 = c2 > 1.17549435e-38f ? c2 : 1.17549435e-38f;
+  auto launch = [&](auto dim, auto f16_, auto qb) {
+    hipLaunchKernelGGL((sink_kernel<decltype(dim)::value, decltype(f16_)::value, decltype(qb)::value>),
+                       dim3((unsigned)(items + g.fills)), dim3(NTH), 0, stream, g);
+  };
+  auto with = [&](auto dim, auto f16_) {
+    narrow ? launch(dim, f16_, std::integral_constant<int, 1>{}) : launch(dim, f16_, std::integral_constant<int, 2>{});
+  };
+  const std::integral_constant<int, 64> d64{};
+  const std::integral_constant<int, 128> d128{};
+  if (a.type == ROWS_F16)
+    a.dim == 64 ? with(d64, std::true_type{}) : with(d128, std::true_type{});
+  else
+    a.dim == 64 ? with(d64, std::false_type{}) : with(d128, std::false_type{});
   NOISE_CHECK_LAUNCH();
   return NOISE_OK;
 }
