@@ -384,10 +384,7 @@ __global__ void __launch_bounds__(64 * NW, 3) attend_kernel(Args g) {
   auto values = [&](int i) {
     const int j0 = block_key(i);
     // the running maximum (lazy) of row lane % 16
-    float mx = -INFINITY;
-#pragma unroll
-    for (int kb = 0; kb < KT; ++kb) mx = fmaxf(mx, fmaxf(fmaxf(sc[kb][0], sc[kb][1]), fmaxf(sc[kb][2], sc[kb][3])));
-    mx = max_rows4(mx);
+    const float mx = max_lanes4(max_scores(sc));
     const bool move = mx * g.c2 > mref * g.c2 + LAZY;
     if (__any(move)) {
       const float mnew = move ? mx : mref;

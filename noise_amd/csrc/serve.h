@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "common.h"
+
 // Codes of a cache: e2m1 (two to a byte, the even channel in the low half) or e4m3. Values of the C ABI's format.
 enum : int { CACHE_FP4 = 0, CACHE_FP8 = 1 };
 // Types of rows handed in or out (values of the C ABI's type).
@@ -127,4 +129,28 @@ constexpr float LAZY = 8.f;  // a running maximum moves only beyond 2^8 of headr
 template <int DIM>
 __device__ __forceinline__ int vswz(int R) {
   return DIM == 64 ? 2 * (((R >> 1) & 1) | ((((R >> 3) ^ R) & 1) << 1)) : 2 * ((R & 3) | (((R >> 3) & 1) << 2));
+}
+
+// max(a, b, c) in one instruction. (fmaxf first quiets each operand with an instruction of its own, as what left the matrix cores
+// could be a signalling NaN for all the compiler knows.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// The largest of a lane's scores, 4 N of them.
+template <int N>
+__device__ __forceinline__ float max_scores(const f32x4 (&s)[N]) {
+  float m = max3(s[0][0], s[0][1], s[0][2]);
+  m = max3(m, s[0][3], s[0][3]);
+#pragma unroll
+  for (int x = 1; x < N; ++x) m = max3(max3(m, s[x][0], s[x][1]), s[x][2], s[x][3]);
+  return m;
+}
+// The same over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float max_lanes4(float x) {
+  const f32pair a = rowpair16(x);
+  const float y = max3(a.lo, a.hi, a.hi);
+  const f32pair b = halves32(y);
+  return max3(b.lo, b.hi, b.hi);
 }

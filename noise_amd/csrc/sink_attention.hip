@@ -12,8 +12,8 @@
 //   Softmax in fp32 with a lazy running maximum; P is rounded once to the operands' type, and its row sums are taken of the rounded
 //   values on the matrix cores (an all-ones operand), so that the rounding cancels in part.
 // Blocks between the sinks and the window are skipped, and a wave skips the blocks none of its queries sees. Blocks seen in part are
-// masked; should such a block hold infinities or NaN among its values, it is multiplied row by row with what the row does not
-// see taken out, since 0 x NaN is not 0.
+// masked. A tile whose output comes out infinite or NaN is computed again row by row, with the values a row does not see taken
+// out of the product, since 0 x NaN is not 0.
 #include <type_traits>
 
 #include "common.h"
@@ -83,44 +83,42 @@ __device__ Tile find_tile(const SinkArgs& a, int id) {
     s0 = min(max(a.starts[b], 0), a.rows);
     return min(max(a.starts[b + 1], s0), a.rows) - s0;
   };
-  long at = j;
+  // (all counts are below the grid's size)
+  int at = j;
   if (!even) {
-    long total = 0;
-    int s0;
+    int total = 0, s0;
     if (a.starts) {
       for (int b0 = 0; b0 < a.n; b0 += 64) total += (rows_of(b0 + lane, s0) + BQ - 1) / BQ;
       for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
       total = uniform(total);
     } else {
-      total = (long)a.n * ((a.T + BQ - 1) / BQ);
+      total = a.n * ((a.T + BQ - 1) / BQ);
     }
     total *= per;
-    const long q = total / 8, r = total % 8;
+    const int q = total / 8, r = total % 8;
     if (j >= q + (x < r)) return t;
-    at = x * q + min((long)x, r) + j;
+    at = x * q + min(x, r) + j;
   }
-  auto take = [&](int s0, int m, long i) {
-    const int tiles = (m + BQ - 1) / BQ, hh = (int)(i / tiles);
+  auto take = [&](int s0, int m, int i) {
+    const int tiles = (m + BQ - 1) / BQ, hh = i / tiles;
     t.found = true;
     t.s0 = s0;
     t.m = m;
-    t.q0 = (tiles - 1 - (int)(i % tiles)) * BQ;
+    t.q0 = (tiles - 1 - i % tiles) * BQ;
     t.h = even ? x * per + hh : hh;
   };
   if (!a.starts) {
-    const long each = (long)((a.T + BQ - 1) / BQ) * per;
-    const long b = at / each;
-    if (b < a.n) take((int)b * a.T, a.T, at % each);
+    const int each = (a.T + BQ - 1) / BQ * per, b = at / each;
+    if (b < a.n) take(b * a.T, a.T, at % each);
     return t;
   }
-  long base = 0;
+  int base = 0;
   for (int b0 = 0; b0 < a.n; b0 += 64) {
     int s0;
-    const int m = rows_of(b0 + lane, s0);
-    const long mine = (long)((m + BQ - 1) / BQ) * per;
-    long upto = mine;
+    const int m = rows_of(b0 + lane, s0), mine = (m + BQ - 1) / BQ * per;
+    int upto = mine;
     for (int o = 1; o < 64; o <<= 1) {
-      const long u = __shfl_up(upto, o, 64);
+      const int u = __shfl_up(upto, o, 64);
       if (lane >= o) upto += u;
     }
     const unsigned long long hits = __ballot(at < base + upto);
@@ -173,183 +171,185 @@ __global__ void __launch_bounds__(NTH, DIM == 64 ? 3 : 2) sink_kernel(Args g) {
   const int lo = first / BKV, sink = min((min(a.sinks, first) + BKV - 1) / BKV, lo), blocks = sink + qlast / BKV - lo + 1;
   auto block_key = [&](int i) { return (i < sink ? i : lo + i - sink) * BKV; };
 
-  // Loads of block i into ring slot buf. Instruction d fills LDS rows RPI d ..; lane L -> row RPI d + L / CH, chunk L % CH.
+  // Loads of block i into ring slot buf. Instruction q of this wave fills LDS rows RPI (DH wave + q) ..; lane L -> row L / CH of
+  // them, chunk L % CH: of K the key kr0 + 16 q (8 q for dim 128), of V the key vr0 + RPI q, each at its swizzled chunk. Rows past
+  // the sequence repeat its last one (no query sees them).
   const int lrow = lane / CH, lchunk = lane % CH;
-  unsigned koffs[DH], voffs[DH];
-#pragma unroll
-  for (int q = 0; q < DH; ++q) {
-    const int R = RPI * (DH * wave + q) + lrow;
-    koffs[q] = 2u * (unsigned)(key_of_row(R) * (int)a.k.ld + 8 * (lchunk ^ kswz<DIM>(R)));
-    voffs[q] = 2u * (unsigned)(R * (int)a.v.ld + 8 * (lchunk ^ vswz<DIM>(R)));
-  }
+  int kr0 = key_of_row(RPI * DH * wave + lrow), vr0 = RPI * DH * wave + lrow;
+  unsigned kc0 = 16 * (lchunk ^ kswz<DIM>(RPI * DH * wave + lrow)), vc0 = 16 * (lchunk ^ vswz<DIM>(vr0));
+  const unsigned kld = 2 * (unsigned)a.k.ld, vld = 2 * (unsigned)a.v.ld;
   auto issue = [&](int i, int buf) {
-    const int j0 = block_key(i);
-    const char *k0 = kp + 2l * j0 * a.k.ld, *v0 = vp + 2l * j0 * a.v.ld;
+    const int j0 = block_key(i), lim = last - j0;
+    // (opaque here and in block(): what is derived from these would be kept in registers over the loop)
+    asm volatile("" : "+v"(kr0), "+v"(vr0), "+v"(kc0), "+v"(vc0));
+    const char *k0 = kp + (long)j0 * kld, *v0 = vp + (long)j0 * vld;
     const char *kd = sk[buf] + DH * wave * 1024, *vd = sv[buf] + DH * wave * 1024;
-    if (j0 + BKV - 1 <= last) {
 #pragma unroll
-      for (int q = 0; q < DH; ++q) dma_x4_s(k0, koffs[q], kd + 1024 * q);
+    for (int q = 0; q < DH; ++q)
+      dma_x4_s(k0, __umul24(min(kr0 + (DIM == 64 ? 16 : 8) * q, lim), kld) + (DIM == 64 ? kc0 : kc0 ^ (64 * q)), kd + 1024 * q);
 #pragma unroll
-      for (int q = 0; q < DH; ++q) dma_x4_s(v0, voffs[q], vd + 1024 * q);
-    } else {  // rows past the sequence repeat its last one (no query sees them)
-#pragma unroll
-      for (int q = 0; q < DH; ++q) {
-        const int R = RPI * (DH * wave + q) + lrow;
-        dma_x4_s(k0, 2u * (unsigned)(min(key_of_row(R), last - j0) * (int)a.k.ld + 8 * (lchunk ^ kswz<DIM>(R))), kd + 1024 * q);
-        dma_x4_s(v0, 2u * (unsigned)(min(R, last - j0) * (int)a.v.ld + 8 * (lchunk ^ vswz<DIM>(R))), vd + 1024 * q);
-      }
-    }
+    for (int q = 0; q < DH; ++q)
+      dma_x4_s(v0, __umul24(min(vr0 + RPI * q, lim), vld) + (vc0 ^ (DIM == 64 ? 64 * q : 128 * (q >> 1))), vd + 1024 * q);
   };
 
   float mref[QB];
   f32x4 o[QB][DT], osum[QB];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    mref[qb] = -INFINITY;
-    osum[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[qb][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
   const x8 ones = {(T)1.f, (T)1.f, (T)1.f, (T)1.f, (T)1.f, (T)1.f, (T)1.f, (T)1.f};
   // fragment i of K tile kb: row 16 kb + r16, chunk 4 i + grp; of V: key 8 grp + t (+ 32 c + 4 x), chunk pair d
-  const int kro = r16 * ROWB + 16 * (grp ^ kswz<DIM>(r16));
+  int kro = r16 * ROWB + 16 * (grp ^ kswz<DIM>(r16));
   const int vrr = 8 * grp + (r16 >> 2);
-  const int vro = vrr * ROWB + 16 * (((lane & 3) >> 1) ^ vswz<DIM>(vrr)) + 8 * (lane & 1);
+  int vro = vrr * ROWB + 16 * (((lane & 3) >> 1) ^ vswz<DIM>(vrr)) + 8 * (lane & 1);
 
-  auto block = [&](int i, auto bufc) {
+  // Block i from ring slot BUF. CAREFUL: with every row's unseen values taken out of the product.
+  auto block = [&](int i, auto bufc, auto carefulc) {
     constexpr int buf = decltype(bufc)::value;
-    if (i + 1 < blocks) issue(i + 1, buf ^ 1);
+    constexpr bool CAREFUL = decltype(carefulc)::value;
     const int j0 = block_key(i);
     const char *kt = sk[buf], *vt = sv[buf];
-    // blocks that this wave's queries see in part, or not at all
-    const bool causal = j0 + BKV - 1 > qw, left = qe - j0 > a.window && j0 + BKV > a.sinks;
-    const bool none = j0 > qe || (qw - (j0 + BKV - 1) > a.window && j0 >= a.sinks);
-    if (!none) {
-      f32x4 s[QB][KB];
+    asm volatile("" : "+v"(kro), "+v"(vro));
+    // blocks that this wave's queries see not at all, or in part
+    if (j0 > qe || (qw - (j0 + BKV - 1) > a.window && j0 >= a.sinks)) return;
+    const bool part = j0 + BKV - 1 > qw || (qe - j0 > a.window && j0 + BKV > a.sinks);
+    f32x4 s[QB][KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        x8 kf[QS];
+    for (int kb = 0; kb < KB; ++kb) {
+      x8 kf[QS];
 #pragma unroll
-        for (int q = 0; q < QS; ++q) kf[q] = *reinterpret_cast<const x8*>(kt + (kro ^ (64 * q)) + 16 * kb * ROWB);
+      for (int q = 0; q < QS; ++q) kf[q] = *reinterpret_cast<const x8*>(kt + (kro ^ (64 * q)) + 16 * kb * ROWB);
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-          s[qb][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int qb = 0; qb < QB; ++qb) {
+        s[qb][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int q = 0; q < QS; ++q) s[qb][kb] = mfma<F16>(kf[q], qf[qb][q], s[qb][kb]);
-        }
+        for (int q = 0; q < QS; ++q) s[qb][kb] = mfma<F16>(kf[q], qf[qb][q], s[qb][kb]);
       }
-      if (causal | left) {
+    }
+    if (part) {
+      // key j0 + 8 grp + t, t a constant, of query j0 + 8 grp + top: seen when 0 <= top - t <= window or t <= top, t < sinks'
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-          const int q = qw + 16 * qb + r16;
+      for (int qb = 0; qb < QB; ++qb) {
+        const int top = qw + 16 * qb + r16 - j0 - 8 * grp;
+        if (j0 >= a.sinks) {
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int j = j0 + 32 * (kb >> 1) + 8 * grp + 4 * (kb & 1) + e;
-              const bool see = (j <= q) & ((q - j <= a.window) | (j < a.sinks));
-              s[qb][kb][e] = see ? s[qb][kb][e] : -INFINITY;
+              const int t = 32 * (kb >> 1) + 4 * (kb & 1) + e;
+              s[qb][kb][e] = (unsigned)(top - t) <= (unsigned)a.window ? s[qb][kb][e] : -INFINITY;
+            }
+        } else {
+          const int few = min(top, a.sinks - 1 - j0 - 8 * grp);
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int t = 32 * (kb >> 1) + 4 * (kb & 1) + e;
+              s[qb][kb][e] = ((unsigned)(top - t) <= (unsigned)a.window) | (t <= few) ? s[qb][kb][e] : -INFINITY;
             }
         }
       }
-      x8 pf[QB][KC];
+    }
+    x8 pf[QB][KC];
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        float mx = fmaxf(s[qb][0][0], s[qb][0][1]);
+    for (int qb = 0; qb < QB; ++qb) {
+      const float mx = max_lanes4(max_scores(s[qb]));
+      const bool move = mx * g.c2 > mref[qb] * g.c2 + LAZY;
+      if (__any(move)) {
+        const float mnew = move ? mx : mref[qb];
+        const float alpha = move ? __builtin_amdgcn_exp2f((mref[qb] - mnew) * g.c2) : 1.f;
+        mref[qb] = mnew;
+        osum[qb] *= alpha;
 #pragma unroll
-        for (int x = 2; x < 4 * KB; x += 2) mx = fmaxf(mx, fmaxf(s[qb][x / 4][x % 4], s[qb][x / 4][x % 4 + 1]));
-        mx = max_rows4(mx);
-        const bool move = mx * g.c2 > mref[qb] * g.c2 + LAZY;
-        if (__any(move)) {
-          const float mnew = move ? mx : mref[qb];
-          const float alpha = move ? __builtin_amdgcn_exp2f((mref[qb] - mnew) * g.c2) : 1.f;
-          mref[qb] = mnew;
-          osum[qb] *= alpha;
+        for (int d = 0; d < DT; ++d) o[qb][d] *= alpha;
+      }
+      const float mc = mref[qb] == -INFINITY ? 0.f : mref[qb] * g.c2;
 #pragma unroll
-          for (int d = 0; d < DT; ++d) o[qb][d] *= alpha;
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          pf[qb][c][x] = (T)__builtin_amdgcn_exp2f(fmaf(s[qb][2 * c + (x >> 2)][x & 3], g.c2, -mc));
+    }
+    auto vfrag = [&](int c, int d) {
+      const char* p = vt + (vro ^ (32 * d)) + 32 * c * ROWB;
+      const x4 l = __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
+      const x4 h = __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(p + 4 * ROWB)));
+      return x8{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+    };
+    if constexpr (!CAREFUL) {
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const x8 vf = vfrag(c, d);
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) o[qb][d] = mfma<F16>(vf, pf[qb][c], o[qb][d]);
         }
-        const float mc = mref[qb] == -INFINITY ? 0.f : mref[qb] * g.c2;
+    } else {
 #pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-            pf[qb][c][x] = (T)__builtin_amdgcn_exp2f(fmaf(s[qb][2 * c + (x >> 2)][x & 3], g.c2, -mc));
-      }
-      auto vfrag = [&](int c, int d) {
-        const char* p = vt + (vro ^ (32 * d)) + 32 * c * ROWB;
-        const x4 l = __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
-        const x4 h = __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(p + 4 * ROWB)));
-        return x8{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
-      };
-      bool odd = false;
-      if (causal | left) {
-        constexpr unsigned EXP = F16 ? 0x7c00u : 0x7f80u;
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const u32x4 v = __builtin_bit_cast(u32x4, vfrag(c, d));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= ((v[e] & EXP) == EXP) | ((v[e] & EXP << 16) == EXP << 16);
-          }
-      }
-      if (!__any(odd)) {
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const x8 vf = vfrag(c, d);
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) o[qb][d] = mfma<F16>(vf, pf[qb][c], o[qb][d]);
-          }
-      } else {
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb)
+      for (int qb = 0; qb < QB; ++qb)
 #pragma unroll 1
-          for (int row = 0; row < 16; ++row) {
-            const int q = qw + 16 * qb + row;
-            int k0 = j0 + 8 * grp;
-            asm volatile("" : "+v"(k0));
-            u32x4 keep[KC];
+        for (int row = 0; row < 16; ++row) {
+          const int top = qw + 16 * qb + row - j0 - 8 * grp, few = min(top, a.sinks - 1 - j0 - 8 * grp);
+#pragma unroll 1
+          for (int c = 0; c < KC; ++c) {
+            u32x4 keep;  // a mask of the fragment's 8 keys 32 c + 8 grp ..
 #pragma unroll
-            for (int c = 0; c < KC; ++c)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                unsigned mk[2];
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                  const int j = k0 + 32 * c + 2 * x + y;
-                  mk[y] = (j <= q) & ((q - j <= a.window) | (j < a.sinks)) ? 0xffffu : 0u;
-                }
-                keep[c][x] = mk[0] | mk[1] << 16;
-              }
+            for (int x = 0; x < 4; ++x) {
+              const int t = 32 * c + 2 * x;
+              const bool one = ((unsigned)(top - t) <= (unsigned)a.window) | (t <= few);
+              const bool two = ((unsigned)(top - t - 1) <= (unsigned)a.window) | (t + 1 <= few);
+              keep[x] = (one ? 0xffffu : 0u) | (two ? 0xffff0000u : 0u);
+            }
+            const x8 pc = c == 0 ? pf[qb][0] : pf[qb][1];
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
               f32x4 add = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int c = 0; c < KC; ++c)
-                add = mfma<F16>(__builtin_bit_cast(x8, __builtin_bit_cast(u32x4, vfrag(c, d)) & keep[c]), pf[qb][c], add);
+              add = mfma<F16>(__builtin_bit_cast(x8, __builtin_bit_cast(u32x4, vfrag(c, d)) & keep), pc, add);
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[qb][d][e] = r16 == row ? o[qb][d][e] + add[e] : o[qb][d][e];
             }
           }
-      }
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) osum[qb] = mfma<F16>(ones, pf[qb][c], osum[qb]);
+        }
     }
-    // block i + 1 has landed for this wave, and the barrier makes every wave's part of it visible and retires slot buf
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) osum[qb] = mfma<F16>(ones, pf[qb][c], osum[qb]);
+  };
+  // Block i + 1 lands in the other slot while block i is computed; then it has landed for this wave, and the barrier makes every
+  // wave's part of it visible and retires block i's slot. (The loads are the only vector memory operations in flight.)
+  auto step = [&](int i, auto bufc, auto carefulc) {
+    if (i + 1 < blocks) issue(i + 1, decltype(bufc)::value ^ 1);
+    block(i, bufc, carefulc);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   };
-
-  issue(0, 0);
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  for (int i = 0; i < blocks; i += 2) {
-    block(i, std::integral_constant<int, 0>{});
-    if (i + 1 < blocks) block(i + 1, std::integral_constant<int, 1>{});
-  }
+  auto pass = [&](auto carefulc) {
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      mref[qb] = -INFINITY;
+      osum[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[qb][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    issue(0, 0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    for (int i = 0; i < blocks; i += 2) {
+      step(i, std::integral_constant<int, 0>{}, carefulc);
+      if (i + 1 < blocks) step(i + 1, std::integral_constant<int, 1>{}, carefulc);
+    }
+  };
+  pass(std::false_type{});
+  // An output that is not finite under a finite sum: infinities or NaN among the values, which in blocks seen in part reach rows that
+  // do not see them (0 x NaN is not 0). All again, row by row.
+  bool odd = false;
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd |= !(fabsf(o[qb][d][e]) < INFINITY);
+  if (__syncthreads_or(odd)) pass(std::true_type{});
 
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
@@ -372,8 +372,8 @@ int sink_attention_launch(const SinkArgs& a, hipStream_t stream) {
       a.kv_heads <= 0 || a.heads % a.kv_heads || a.window < 0 || a.sinks < 0 || !(a.scale >= 0.f) || a.scale > 3.4e38f ||
       a.n <= 0 || a.rows <= 0 || (!a.starts && (a.T <= 0 || (long)a.n * a.T != a.rows)))
     return NOISE_EINVAL;
-  // (byte offsets inside a 64-key block are 32-bit)
-  if (a.k.ld > (1 << 24) || a.v.ld > (1 << 24)) return NOISE_ENOTSUP;
+  // (byte strides of 24 bits: offsets inside a 64-key block are 24-bit products)
+  if (a.k.ld >= (1 << 23) || a.v.ld >= (1 << 23)) return NOISE_ENOTSUP;
   // tiles: of queries, at most one begun by every sequence beside the full ones; the GPU counts them
   auto groups = [&](int bq) {
     const long tiles = a.starts ? a.rows / bq + (a.n < a.rows ? a.n : a.rows) : (long)a.n * ((a.T + bq - 1) / bq);
