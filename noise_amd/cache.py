@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import ROW_TYPES, _ptr, _stream, heads_rows, mask_args, no_grad_rows, one_device, output_rows, sequence_starts
+from .ops import ROW_TYPES, _ptr, heads_rows, launch, mask_args, no_grad_rows, one_device, output_rows, sequence_starts
 
 FORMATS = {'fp4': _lib.CACHE_FP4, 'fp8': _lib.CACHE_FP8}
 
@@ -51,6 +51,8 @@ class KVCache:
         self.keys, self.key_scales, self.values, self.value_scales = keys, key_scales, values, value_scales
         self._desc = _lib.Cache(keys.data_ptr(), key_scales.data_ptr(), values.data_ptr(), value_scales.data_ptr(), self.pages,
                                 self.page_size, self.kv_heads, self.dim, FORMATS[self.format])
+        self._ptr = ctypes.addressof(self._desc)
+        self._sizes = {}  # attend's workspace bytes by the shape of a call
 
     @classmethod
     def zeros(cls, pages, kv_heads=8, dim=64, page_size=64, format='fp4', device='cuda'):
@@ -66,7 +68,7 @@ class KVCache:
         one_device(self.keys, table, lengths)
         if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError('table must be an int32 tensor [sequences, pages of a sequence] with contiguous rows')
-        n = table.shape[0]
+        n, pages = table.shape
         if lengths.dtype != torch.int32 or tuple(lengths.shape) != (n,) or not lengths.is_contiguous():
             raise ValueError(f'lengths must be a contiguous int32 vector of {n} entries')
         if starts is None:
@@ -74,8 +76,7 @@ class KVCache:
                 raise ValueError(f'{rows} rows of {n} sequences need starts')
         elif sequence_starts(starts, self.device) != n:
             raise ValueError(f'starts must have {n + 1} entries')
-        pages = table.shape[1]
-        return _lib.Sequences(_ptr(table), max(table.stride(0), pages), pages, lengths.data_ptr(), _ptr(starts), n, rows)
+        return _lib.Sequences(table.data_ptr(), max(table.stride(0), pages), pages, lengths.data_ptr(), _ptr(starts), n, rows)
 
     def write(self, k, v, table, lengths, starts=None):
         """Quantises the rows k and v [n, kv_heads, dim] (bf16, fp16 or fp32, any strides) into their places. The places of one
@@ -91,9 +92,7 @@ class KVCache:
             return
         k, kp, kl, kh = heads_rows(k)
         v, vp, vl, vh = heads_rows(v)
-        with torch.cuda.device(self.device):
-            _lib.call('noise_cache_write', ctypes.addressof(self._desc), ctypes.addressof(seqs), kp, kl, kh, vp, vl, vh,
-                      ROW_TYPES[k.dtype], _stream())
+        launch(self.device, 'noise_cache_write', self._ptr, ctypes.addressof(seqs), kp, kl, kh, vp, vl, vh, ROW_TYPES[k.dtype])
 
     def read(self, table, lengths, starts=None, rows=None, dtype=torch.bfloat16):
         """(k, v) [rows, kv_heads, dim]: the cached values at the rows' places, rounded to dtype (bf16, fp16 or fp32). With starts,
@@ -111,11 +110,11 @@ class KVCache:
         shape = (rows, self.kv_heads, self.dim)
         if not seqs.sequences:
             return torch.zeros(shape, device=self.device, dtype=dtype), torch.zeros(shape, device=self.device, dtype=dtype)
-        k, v = (torch.empty(shape, device=self.device, dtype=dtype) for _ in range(2))
+        k = torch.empty(shape, device=self.device, dtype=dtype)
+        v = torch.empty_like(k)
         if rows:
-            with torch.cuda.device(self.device):
-                _lib.call('noise_cache_read', ctypes.addressof(self._desc), ctypes.addressof(seqs), k.data_ptr(), v.data_ptr(),
-                          ROW_TYPES[dtype], _stream())
+            launch(self.device, 'noise_cache_read', self._ptr, ctypes.addressof(seqs), k.data_ptr(), v.data_ptr(),
+                   ROW_TYPES[dtype])
         return k, v
 
     def attend(self, q, table, lengths, starts=None, window=None, sinks=0, scale=None, out=None):
@@ -138,10 +137,14 @@ class KVCache:
             return y.zero_() if fill else y
         heads = q.shape[1]
         q, qp, ql, qh = heads_rows(q)
-        cache, call = ctypes.addressof(self._desc), ctypes.addressof(seqs)
-        with torch.cuda.device(self.device):
-            size = _lib.size_query('noise_cache_attend_workspace_size', cache, call, heads, window, sinks)
-            ws = torch.empty(size, device=self.device, dtype=torch.uint8) if size else None
-            _lib.call('noise_cache_attend', cache, call, qp, ql, qh, ROW_TYPES[q.dtype], heads, window, sinks, scale,
-                      y.data_ptr(), fill, _ptr(ws), size, _stream())
+        call = ctypes.addressof(seqs)
+        shape = (seqs.sequences, seqs.rows, seqs.table_pages, starts is None, heads)
+        size = self._sizes.get(shape)
+        if size is None:
+            if len(self._sizes) >= 256:
+                self._sizes.clear()
+            size = self._sizes[shape] = _lib.size_query('noise_cache_attend_workspace_size', self._ptr, call, heads)
+        ws = torch.empty(size, device=self.device, dtype=torch.uint8) if size else None
+        launch(self.device, 'noise_cache_attend', self._ptr, call, qp, ql, qh, ROW_TYPES[q.dtype], heads, window, sinks, scale,
+               y.data_ptr(), fill, _ptr(ws), size)
         return y

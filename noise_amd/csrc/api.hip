@@ -713,15 +713,12 @@ int noise_cache_read(const noise_cache_t* cache, const noise_sequences_t* seqs, 
   return cache_read_launch(c, s, k, v, type, static_cast<hipStream_t>(stream));
 }
 
-int noise_cache_attend_workspace_size(const noise_cache_t* cache, const noise_sequences_t* seqs, int heads, int window,
-                                      int sinks, size_t* bytes) {
+int noise_cache_attend_workspace_size(const noise_cache_t* cache, const noise_sequences_t* seqs, int heads, size_t* bytes) {
   Cache c;
   Sequences s;
   if (!bytes || !copy_cache(cache, seqs, &c, &s)) return NOISE_EINVAL;
   AttendArgs a{};
   a.heads = heads;
-  a.window = window;
-  a.sinks = sinks;
   return cache_attend_workspace(c, s, a, bytes);
 }
 

@@ -120,9 +120,22 @@ ROW_TYPES = {torch.bfloat16: _lib.ROWS_BF16, torch.float16: _lib.ROWS_F16, torch
 NO_WINDOW = 2 ** 31 - 1
 
 
+def launch(dev, name, *args):
+    """Calls an entry point on device dev, on its current stream (the last argument)."""
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+
 def no_grad_rows(*tensors):
     """The serving operators are forward-only: refuse a tensor whose gradient a caller would expect."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if not t.requires_grad:
+            continue
         raise RuntimeError('the serving operators have no backward pass: call them under torch.no_grad() or detach the inputs')
 
 
@@ -130,7 +143,7 @@ def one_device(*tensors):
     """The CUDA device that all of them are on."""
     dev = tensors[0].device
     for t in tensors:
-        if t.device.type != 'cuda':
+        if not t.is_cuda:
             raise ValueError('the operands must be CUDA tensors (no CPU path)')
         if t.device != dev:
             raise ValueError(f'the operands are on different devices ({dev} and {t.device})')
@@ -142,12 +155,13 @@ def heads_rows(t):
     where the channels are contiguous and rows and heads start at 16-byte addresses, else from a contiguous copy."""
     unit = 16 // t.element_size()
     n, heads, dim = t.shape
+    ld, hs, one = t.stride()
     # (the stride of a dimension of one entry means nothing)
-    ld, hs = t.stride(0) if n > 1 else 0, t.stride(1) if heads > 1 else 0
-    if t.stride(2) != 1 or ld % unit or hs % unit or t.data_ptr() % 16:
+    ld, hs, p = ld if n > 1 else 0, hs if heads > 1 else 0, t.data_ptr()
+    if one != 1 or ld % unit or hs % unit or p % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-        ld, hs = heads * dim, dim
-    return t, t.data_ptr(), ld, hs
+        ld, hs, p = heads * dim, dim, t.data_ptr()
+    return t, p, ld, hs
 
 
 def mask_args(window, sinks, scale, dim):
@@ -166,14 +180,15 @@ def sequence_starts(starts, dev):
     """Checks the packed rows' starts and returns the number of sequences."""
     if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() < 1 or not starts.is_contiguous():
         raise ValueError('starts must be a contiguous int32 vector of sequences + 1 entries')
-    one_device(torch.empty(0, device=dev), starts)
+    if starts.device != dev:
+        raise ValueError(f'starts must be on {dev}, got {starts.device}')
     return starts.numel() - 1
 
 
 def output_rows(out, like, dev):
     """The output [n, heads, dim] and whether rows of no sequence are to be zeroed (not in a tensor the caller gave)."""
     if out is None:
-        return torch.empty(like.shape, device=dev, dtype=like.dtype), 1
+        return torch.empty_like(like, memory_format=torch.contiguous_format), 1
     if out.shape != like.shape or out.dtype != like.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f'out must be a contiguous {like.dtype} tensor of shape {tuple(like.shape)} beside q, 16-byte aligned')
     no_grad_rows(out)
@@ -218,7 +233,6 @@ def sink_attention(q, k, v, starts=None, window=None, sinks=0, scale=None, out=N
     q, qp, ql, qh = heads_rows(q)
     k, kp, kl, kh = heads_rows(k)
     v, vp, vl, vh = heads_rows(v)
-    with torch.cuda.device(dev):
-        _lib.call('noise_sink_attention', qp, ql, qh, kp, kl, kh, vp, vl, vh, _ptr(starts), n, rows, T, heads, kv, dim,
-                  ROW_TYPES[q.dtype], window, sinks, scale, y.data_ptr(), fill, _stream())
+    launch(dev, 'noise_sink_attention', qp, ql, qh, kp, kl, kh, vp, vl, vh, _ptr(starts), n, rows, T, heads, kv, dim,
+           ROW_TYPES[q.dtype], window, sinks, scale, y.data_ptr(), fill)
     return y
