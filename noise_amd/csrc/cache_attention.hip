@@ -14,10 +14,11 @@
 // fp16 queries and their probabilities enter as two bf16 terms (hi + lo: 16 significant bits, fp16 has 11); bf16 queries are
 // exact and their probabilities are rounded once to bf16, the type of the output.
 //
-// Work is cut on the GPU from the sequences' lengths, which the host does not know: all blocks of all sequences are shared out in
-// chunks of equal length, at most TARGET workgroups' worth, a workgroup taking one chunk of one sequence and kv head, its
-// waves block by block in turn. The waves join in LDS; where a sequence has several chunks, their sums meet in a second kernel,
-// in chunk order (the same bits every time).
+// Work is cut on the GPU from the sequences' lengths, which the host does not know. The rounds (a block for each wave) of all
+// tiles, kv head by kv head, form one line, and each of the workgroups that fill the GPU once takes an equal stretch of it:
+// every workgroup has the same to do whatever the lengths. A stretch may hold the end of one tile, whole tiles and
+// the beginning of another; the waves join in LDS, and where a tile is spread over several workgroups their sums meet in a second
+// kernel, in order (the same bits every time). Tables that name few keys go without it: a workgroup a tile.
 #include <type_traits>
 
 #include "common.h"
@@ -67,8 +68,9 @@ struct Cut {
 struct Plan {
   int group;        // query heads of a kv head
   int block_shift;  // log2 of a block's keys
-  int target;       // chunks wanted per kv head
-  int waves;        // a chunk has at least this many blocks
+  int cap;          // positions that a table names
+  int groups;       // workgroups that share the line, or 0: a workgroup a tile
+  int waves;        // of a workgroup: the blocks of a round
 };
 
 __device__ __forceinline__ int first_key(int pos, int window) { return pos > window ? pos - window : 0; }
@@ -85,7 +87,7 @@ __device__ __forceinline__ Range range_of(int p0, int p1, int window, int sinks,
   return Range{sink, lo, sink + (p1 >> shift) - lo + 1};
 }
 
-__device__ __forceinline__ Cut cut_of(const Sequences& s, const Plan& p, int page_shift, int window, int sinks, int b, int& s0) {
+__device__ __forceinline__ Cut cut_of(const Sequences& s, const Plan& p, int window, int sinks, int b, int& s0) {
   Cut c{0, 0, 0, 0};
   s0 = 0;
   if (b >= s.n) return c;
@@ -98,10 +100,10 @@ __device__ __forceinline__ Cut cut_of(const Sequences& s, const Plan& p, int pag
     s1 = b + 1;
   }
   c.m = s1 - s0;
-  c.len = s.lengths[b];
-  c.tiles = (int)(((long)c.m * p.group + RT - 1) / RT);
+  c.len = max(s.lengths[b], 0);
+  c.tiles = (c.m * p.group + RT - 1) / RT;
   // (positions past the table hold nothing: the rows there are NaN, and the others end in front of it)
-  const int last = (int)min((long)c.len, (long)s.table_pages << page_shift) - 1;
+  const int last = min(c.len, p.cap) - 1;
   if (c.m > 0 && last >= 0) {
     // a tile's rows are at most `span` tokens; its range is at most that of the last ones, and a block more by alignment
     const int span = min(c.m, (RT + p.group - 1) / p.group + 1);
@@ -110,39 +112,66 @@ __device__ __forceinline__ Cut cut_of(const Sequences& s, const Plan& p, int pag
   return c;
 }
 
+// The line: `units` rounds per kv head (a tile that sees no key counts as one), `share` of them to a workgroup.
+struct Line {
+  int units, share;
+};
+// A tile on the line of its kv head: `at` its first round, `rounds` their number; or, without a line, `at` its number.
 struct Work {
-  int b, s0, m, len, tile, split, splits, chunk, first;
+  int b, s0, m, len, tile, rounds, at;
   bool found;
 };
 
-// Finds chunk `item` of the call (row < 0), or the sequence of row `row` with its first chunk. Whole waves.
-__device__ Work find_work(const Sequences& s, const Plan& p, int page_shift, int window, int sinks, int item, int row) {
+// The cuts of up to 64 sequences in LDS, for the tiles after the first (every wave writes the same values).
+struct Kept {
+  int s0[64], m[64], len[64], blocks[64], tiles[64];
+};
+
+__device__ __forceinline__ int rounds_of(const Plan& p, const Cut& c) { return max((c.blocks + p.waves - 1) / p.waves, 1); }
+
+// (the host keeps all rounds of a call below 2^31)
+__device__ Line line_of(const Sequences& s, const Plan& p, int kv_heads, int window, int sinks, Kept& kept) {
   const int lane = threadIdx.x & 63;
-  long total = 0;
-  Cut c{};
-  int s0 = 0;
+  int total = 0;
   for (int b0 = 0; b0 < s.n; b0 += 64) {
-    c = cut_of(s, p, page_shift, window, sinks, b0 + lane, s0);
-    total += (long)c.tiles * c.blocks;
+    int s0;
+    const Cut c = cut_of(s, p, window, sinks, b0 + lane, s0);
+    total += c.tiles * rounds_of(p, c);
+    if (s.n <= 64) {
+      kept.s0[lane] = s0;
+      kept.m[lane] = c.m;
+      kept.len[lane] = c.len;
+      kept.blocks[lane] = c.blocks;
+      kept.tiles[lane] = c.tiles;
+    }
   }
   for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
   total = uniform(total);
-  long chunk = (total + p.target - 1) / p.target;
-  chunk = max(chunk, (long)p.waves);
-  chunk = (chunk + p.waves - 1) / p.waves * p.waves;
+  return Line{total, (total * kv_heads + p.groups - 1) / p.groups};
+}
+
+// The tile that holds round `unit` of a kv head's line (row < 0), or the one of row `row` and head `head` of its group. Whole waves.
+__device__ Work find_work(const Sequences& s, const Plan& p, int window, int sinks, int unit, int row, int head, const Kept& kept) {
+  const int lane = threadIdx.x & 63;
   Work w{};
-  w.chunk = (int)min(chunk, 0x7fffffffl);
-  long base = 0;
+  int base = 0;
   for (int b0 = 0; b0 < s.n; b0 += 64) {
-    if (s.n > 64) c = cut_of(s, p, page_shift, window, sinks, b0 + lane, s0);
-    const int splits = max(1, (c.blocks + w.chunk - 1) / w.chunk);
-    const long mine = (long)c.tiles * splits;
-    long upto = mine;
+    int s0;
+    Cut c;
+    if (p.groups && s.n <= 64) {
+      s0 = kept.s0[lane];
+      c = Cut{kept.m[lane], kept.len[lane], kept.blocks[lane], kept.tiles[lane]};
+    } else {
+      c = cut_of(s, p, window, sinks, b0 + lane, s0);
+    }
+    const int each = p.groups ? rounds_of(p, c) : 1;
+    const int mine = c.tiles * each;
+    int upto = mine;
     for (int o = 1; o < 64; o <<= 1) {
-      const long t = __shfl_up(upto, o, 64);
+      const int t = __shfl_up(upto, o, 64);
       if (lane >= o) upto += t;
     }
-    const bool hit = row >= 0 ? row >= s0 && row < s0 + c.m : item < base + upto;
+    const bool hit = row >= 0 ? row >= s0 && row < s0 + c.m : unit < base + upto;
     const unsigned long long hits = __ballot(hit);
     if (hits) {
       const int k = __builtin_ctzll(hits);
@@ -151,10 +180,10 @@ __device__ Work find_work(const Sequences& s, const Plan& p, int page_shift, int
       w.s0 = uniform(s0, k);
       w.m = uniform(c.m, k);
       w.len = uniform(c.len, k);
-      w.splits = uniform(splits, k);
-      w.first = (int)base + uniform((int)(upto - mine), k);
-      w.tile = (item - w.first) / w.splits;
-      w.split = (item - w.first) % w.splits;
+      w.rounds = uniform(each, k);
+      const int first = base + uniform(upto - mine, k);
+      w.tile = row >= 0 ? ((row - w.s0) * p.group + head) / RT : (unit - first) / w.rounds;
+      w.at = first + w.tile * w.rounds;
       return w;
     }
     base += uniform(upto, 63);
@@ -168,39 +197,53 @@ struct Args {
   AttendArgs a;
   Plan p;
   float c2;         // scale in base-2 units
-  int items, fills;  // workgroups of chunks, workgroups that zero rows
-  float* part;      // [items, RT, dim] sums of chunks, under the maxima of
-  float2* ml;       // [items, RT] (maximum, sum)
+  int items, fills;  // workgroups of tiles or stretches, workgroups that zero rows
+  float* part;      // [groups, 2, RT, dim] sums of a stretch's first and of its last tile, where others hold more of them,
+  float2* ml;       // [groups, 2, RT] under these maxima, with these sums of probabilities
 };
 
 // WIDE: pages hold whole blocks. F16: fp16 queries (two bf16 terms). NW waves.
 template <int DIM, int FMT, bool F16, bool WIDE, int NW>
-__global__ void __launch_bounds__(64 * NW, 3) attend_kernel(Args g) {
+__global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : 3) attend_kernel(Args g) {
   using G = Geo<DIM, FMT>;
   constexpr int BK = G::BK, KT = G::KT, KC = G::KC, DT = G::DT, QS = G::QS, KW = G::KW, VW = G::VW, VN = G::VN;
   constexpr int SHIFT = DIM == 64 ? 6 : 5;
   __shared__ __attribute__((aligned(1024))) char sv[NW * G::TILE];
   __shared__ float2 sml[NW][RT];
+  __shared__ Kept kept;
   const Cache& c = g.c;
   const Sequences& s = g.s;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r16 = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   if ((int)blockIdx.x >= g.items) {
     fill_rows(s.starts, s.n, s.rows, g.a.y, g.a.heads * DIM, 64 * NW, blockIdx.x - g.items, g.fills);
     return;
   }
-  const int kh = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads;
-  const Work w = find_work(s, g.p, c.page_shift, g.a.window, g.a.sinks, item, -1);
+  char* vt = sv + wave * G::TILE;
+  const int page_mask = (1 << c.page_shift) - 1;
+  Line line{};
+  int unit = 0, end = 0;
+  if (g.p.groups) {
+    line = line_of(s, g.p, c.kv_heads, g.a.window, g.a.sinks, kept);
+    unit = blockIdx.x * line.share;
+    end = min(unit + line.share, line.units * c.kv_heads);
+    if (unit >= end) return;
+  }
+#pragma unroll 1
+  for (bool more = true; more;) {
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // (opaque: what a lane derives from it would be kept in registers over the loop)
+  const int lane = tid & 63, r16 = lane & 15, grp = lane >> 4;
+  const int kh = g.p.groups ? unit / line.units : blockIdx.x % c.kv_heads;
+  const Work w = find_work(s, g.p, g.a.window, g.a.sinks, g.p.groups ? unit - kh * line.units : blockIdx.x / c.kv_heads, -1, 0,
+                           kept);
   if (!w.found) return;
-  const int G_ = g.p.group, f0 = w.tile * RT, fn = min(RT, (int)min((long)w.m * G_ - f0, (long)RT));
-  const int t0 = f0 / G_, t1 = (f0 + fn - 1) / G_;                    // the tile's tokens
-  const long p0 = (long)w.len - w.m + t0, p1 = (long)w.len - w.m + t1;  // their positions
-  const long cap = (long)s.table_pages << c.page_shift;                 // positions that the table names
-  const int pmin = (int)max(p0, -1l), pmax = (int)max(min(p1, cap - 1), -1l);
+  const int G_ = g.p.group, f0 = w.tile * RT, fn = min(RT, w.m * G_ - f0), back = w.len - w.m;
+  const int p0 = back + f0 / G_, p1 = back + (f0 + fn - 1) / G_;  // positions of the tile's first and last row
+  const int pmin = max(p0, -1), pmax = max(min(p1, g.p.cap - 1), -1);
   // this lane's row
   const int f = f0 + r16, tok = f / G_;
   const bool live = r16 < fn;
-  const int pos = live ? (int)max((long)w.len - w.m + tok, -1l) : -1;
+  const int pos = live ? max(back + tok, -1) : -1;
 
   // Q fragments (B operand): row lane % 16, channels (lane / 16) DIM / 4 + 8 i ..
   bf16x8 qh[QS], ql[F16 ? QS : 1];
@@ -229,11 +272,20 @@ __global__ void __launch_bounds__(64 * NW, 3) attend_kernel(Args g) {
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const Range rg = pmax >= 0 && p0 < cap ? range_of(pmin, pmax, g.a.window, g.a.sinks, SHIFT) : Range{0, 0, 0};
-  const int i0 = w.split * w.chunk, i1 = (int)min((long)i0 + w.chunk, (long)rg.blocks);
+  const Range rg = pmax >= 0 && p0 < g.p.cap ? range_of(pmin, pmax, g.a.window, g.a.sinks, SHIFT) : Range{0, 0, 0};
+  // this workgroup's blocks i0 .. i1 of the tile; `alone` when no other has any
+  int i0 = 0, i1 = rg.blocks, slot = 0;
+  bool alone = true;
+  if (g.p.groups) {
+    const int from = kh * line.units + w.at, stop = min(end, from + w.rounds);
+    alone = unit == from && stop == from + w.rounds;
+    slot = 2 * blockIdx.x + (unit != (int)blockIdx.x * line.share);
+    i0 = (unit - from) * NW;
+    i1 = min((stop - from) * NW, rg.blocks);
+    unit = stop;
+  }
+  more = g.p.groups && unit < end;
   const int* table = s.table + (long)w.b * s.table_ld;
-  char* vt = sv + wave * G::TILE;
-  const int page_mask = (1 << c.page_shift) - 1;
 
   // row lane % 16 of K tile kb is key 32 (kb / 2) + 4 (kb % 2) + krow0 of the block; piece n of V is 32 channels, vgr, of key
   // n * 64 / GROUPS + vrow0
@@ -505,13 +557,13 @@ __global__ void __launch_bounds__(64 * NW, 3) attend_kernel(Args g) {
       sum[0] = fmaf(wt, v.x, sum[0]), sum[1] = fmaf(wt, v.y, sum[1]);
       sum[2] = fmaf(wt, v.z, sum[2]), sum[3] = fmaf(wt, v.w, sum[3]);
     }
-    if (w.splits > 1) {
-      *reinterpret_cast<f32x4*>(g.part + ((long)blockIdx.x * RT + row) * DIM + d) = sum;
-      if (d == 0) g.ml[(long)blockIdx.x * RT + row] = make_float2(M, L);
+    if (!alone) {
+      *reinterpret_cast<f32x4*>(g.part + ((long)slot * RT + row) * DIM + d) = sum;
+      if (d == 0) g.ml[(long)slot * RT + row] = make_float2(M, L);
       continue;
     }
     const int ff = f0 + row;
-    const float inv = (long)w.len - w.m + ff / G_ >= cap ? __uint_as_float(0x7fc00000u) : L == 0.f ? 0.f : 1.f / L;
+    const float inv = back + ff / G_ >= g.p.cap ? __uint_as_float(0x7fc00000u) : L == 0.f ? 0.f : 1.f / L;
     const long at = ((long)(w.s0 + ff / G_) * g.a.heads + kh * G_ + ff % G_) * DIM + d;
     uint16_t* dst = static_cast<uint16_t*>(g.a.y) + at;
     union {
@@ -527,31 +579,37 @@ __global__ void __launch_bounds__(64 * NW, 3) attend_kernel(Args g) {
         out.b[x] = to_bf16(sum[x] * inv);
     *reinterpret_cast<uint2*>(dst) = out.u;
   }
+  if (more) __syncthreads();  // (the tiles are read before the next stretch writes them)
+  }
 }
 
-// y of the rows whose sequence has several chunks: one workgroup a row and head, its waves taking chunks in turn.
+// y of the rows whose tile several workgroups share: one workgroup a row and head, its waves taking the others' sums in turn.
 template <int DIM, bool F16>
 __global__ void __launch_bounds__(256) join_kernel(Args g) {
   constexpr int NW = 4, PER = DIM / 64;
   __shared__ float so[NW][DIM], sl[NW];
+  __shared__ Kept kept;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x / g.a.heads, h = blockIdx.x % g.a.heads, kh = h / g.p.group;
-  const Work w = find_work(g.s, g.p, g.c.page_shift, g.a.window, g.a.sinks, 0, row);
-  if (!w.found || w.splits == 1) return;
-  const int f = (row - w.s0) * g.p.group + h % g.p.group;
-  const long stride = (long)g.c.kv_heads * RT, at = ((long)(w.first + f / RT * w.splits) * g.c.kv_heads + kh) * RT + f % RT;
-  if (at + (w.splits - 1) * stride >= (long)g.items * RT) return;  // (only starts that overlap name more chunks than there are)
+  const Line line = line_of(g.s, g.p, g.c.kv_heads, g.a.window, g.a.sinks, kept);
+  const Work w = find_work(g.s, g.p, g.a.window, g.a.sinks, 0, row, h % g.p.group, kept);
+  if (!w.found) return;
+  const int from = kh * line.units + w.at, first = from / line.share, last = (from + w.rounds - 1) / line.share;
+  if (first == last) return;
+  const int n = last - first + 1, r = ((row - w.s0) * g.p.group + h % g.p.group) % RT;
+  // the tile is the last of its first workgroup's stretch (its only one, if it begins there), and the first of the others'
+  auto at = [&](int x) { return (2l * (first + x) + (x == 0 && from != first * line.share)) * RT + r; };
   float M = -INFINITY;
-  for (int x = lane; x < w.splits; x += 64) M = fmaxf(M, g.ml[at + x * stride].x);
+  for (int x = lane; x < n; x += 64) M = fmaxf(M, g.ml[at(x)].x);
   for (int q = 32; q; q >>= 1) M = fmaxf(M, __shfl_xor(M, q, 64));
   float L = 0.f, o[PER] = {};
 #pragma unroll 8
-  for (int x = wave; x < w.splits; x += NW) {
-    const float2 ml = g.ml[at + x * stride];
+  for (int x = wave; x < n; x += NW) {
+    const float2 ml = g.ml[at(x)];
     const float wt = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * g.c2);
     L = fmaf(wt, ml.y, L);
 #pragma unroll
-    for (int d = 0; d < PER; ++d) o[d] = fmaf(wt, g.part[(at + x * stride) * DIM + lane + 64 * d], o[d]);
+    for (int d = 0; d < PER; ++d) o[d] = fmaf(wt, g.part[at(x) * DIM + lane + 64 * d], o[d]);
   }
 #pragma unroll
   for (int d = 0; d < PER; ++d) so[wave][lane + 64 * d] = o[d];
@@ -560,7 +618,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args g) {
   if (threadIdx.x < DIM) {
     const int d = threadIdx.x;
     const float l = (sl[0] + sl[1]) + (sl[2] + sl[3]), v = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
-    const bool past = (long)w.len - w.m + (row - w.s0) >= (long)g.s.table_pages << g.c.page_shift;
+    const bool past = w.len - w.m + (row - w.s0) >= g.p.cap;
     const float y = past ? __uint_as_float(0x7fc00000u) : l == 0.f ? 0.f : v / l;
     const long dst = (long)blockIdx.x * DIM + d;
     if constexpr (F16)
@@ -570,44 +628,49 @@ __global__ void __launch_bounds__(256) join_kernel(Args g) {
   }
 }
 
-constexpr int WAVES = 4;
-constexpr int TARGET = 2048;  // workgroups wanted
-
 bool bad_attend(const Cache& c, const Sequences& s, const AttendArgs& a) {
   return bad_cache(c, s) || a.heads <= 0 || a.heads > 1024 || a.heads % c.kv_heads || a.window < 0 || a.sinks < 0;
 }
 
-// How a call is cut: upper bounds of what the GPU finds from the lengths.
+// How a call is cut, by upper bounds of what the GPU finds from the lengths.
 struct Shape {
   Plan p;
   long items;  // workgroups
-  bool join;   // whether a sequence can have several chunks
 };
 Shape shape_of(const Cache& c, const Sequences& s, const AttendArgs& a) {
   Shape r{};
   r.p.group = a.heads / c.kv_heads;
   r.p.block_shift = c.dim == 64 ? 6 : 5;
-  r.p.waves = WAVES;
-  r.p.target = (TARGET + c.kv_heads - 1) / c.kv_heads;
-  // tiles: at most one begun by every sequence beside the full ones; chunks: at most one begun by every tile beside the target
+  const long cap = (long)s.table_pages << c.page_shift;
+  r.p.cap = (int)(cap < 0x7fffffffL ? cap : 0x7fffffffL);
+  // tiles: at most one begun by every sequence beside the full ones; no tile sees more blocks than the table names (and one more
+  // by alignment)
   const long full = (long)s.rows * r.p.group / RT;
-  const long tiles = s.starts ? full + (s.n < s.rows ? s.n : s.rows) : (long)s.rows * ((r.p.group + RT - 1) / RT);
-  const long keys = (long)s.table_pages << c.page_shift;
-  const long blocks = (keys >> r.p.block_shift) + 3;  // (no range has more, its alignment included)
-  const long chunks = tiles * ((blocks + r.p.waves - 1) / r.p.waves);
-  r.items = (chunks < r.p.target + tiles ? chunks : r.p.target + tiles) * c.kv_heads;
-  r.join = blocks > r.p.waves;
+  const long tiles = (s.starts ? full + (s.n < s.rows ? s.n : s.rows) : (long)s.rows * ((r.p.group + RT - 1) / RT)) * c.kv_heads;
+  const long blocks = (r.p.cap >> r.p.block_shift) + 2, fill = 3l * num_cus();
+  // A workgroup a tile, and no second kernel, where a table names so few keys that this costs no more than sharing them out (a
+  // round takes about 1.4 us): 11 blocks of 8 heads on eight waves 8.2 us, shared 7.3 + 4.4; 64 sequences of 33 blocks 20.8,
+  // shared 23.8 + 4.8; but one of 63 blocks 17.5, shared 7.3 + 5.7. Also where there are many tiles, or more rounds than fit.
+  r.items = tiles;
+  r.p.waves = 4;
+  if (blocks <= 34 && tiles <= num_cus()) {
+    r.p.waves = 8;
+    return r;
+  }
+  if (blocks <= 18 || (blocks <= 66 && tiles >= fill / 2) || tiles >= 32 * fill || tiles * blocks > 0x3fffffffL) return r;
+  const long most = tiles * ((blocks + r.p.waves - 1) / r.p.waves);
+  r.items = r.p.groups = (int)(most < fill ? most : fill);
   return r;
 }
 
-size_t part_bytes(const Cache& c, const Shape& r) { return (size_t)r.items * RT * c.dim * 4; }
+size_t part_bytes(const Cache& c, const Shape& r) { return (size_t)r.p.groups * 2 * RT * c.dim * 4; }
 
 }  // namespace
 
 int cache_attend_workspace(const Cache& c, const Sequences& s, const AttendArgs& a, size_t* bytes) {
   if (bad_attend(c, s, a)) return NOISE_EINVAL;
   const Shape r = shape_of(c, s, a);
-  *bytes = r.join ? part_bytes(c, r) + (size_t)r.items * RT * 8 : 0;
+  *bytes = part_bytes(c, r) + (size_t)r.p.groups * 2 * RT * 8;
   return NOISE_OK;
 }
 
@@ -625,7 +688,7 @@ int cache_attend_launch(const Cache& c, const Sequences& s, const AttendArgs& a,
   const float c2 = a.scale * 1.4426950408889634f;
   g.c2 = c2 > 1.17549435e-38f ? c2 : 1.17549435e-38f;
   g.fills = a.fill && s.starts ? 32 : 0;
-  if (r.items + g.fills > 0x7fffffffL || (r.join && (long)s.rows * a.heads > 0x7fffffffL)) return NOISE_ENOTSUP;
+  if ((long)s.rows * a.heads > 0x7fffff00L || r.items + g.fills > 0x7fffffffL) return NOISE_ENOTSUP;
   g.items = (int)r.items;
   g.part = static_cast<float*>(ws);
   g.ml = ws ? reinterpret_cast<float2*>(static_cast<char*>(ws) + part_bytes(c, r)) : nullptr;
@@ -633,7 +696,11 @@ int cache_attend_launch(const Cache& c, const Sequences& s, const AttendArgs& a,
   auto launch = [&](auto dim, auto fmt, auto f16_, auto wide_) {
     constexpr int D = decltype(dim)::value, F = decltype(fmt)::value;
     constexpr bool H = decltype(f16_)::value, W = decltype(wide_)::value;
-    hipLaunchKernelGGL((attend_kernel<D, F, H, W, WAVES>), dim3((unsigned)(g.items + g.fills)), dim3(64 * WAVES), 0, stream, g);
+    const dim3 grid((unsigned)(g.items + g.fills));
+    if (r.p.waves == 8)
+      hipLaunchKernelGGL((attend_kernel<D, F, H, W, 8>), grid, dim3(512), 0, stream, g);
+    else
+      hipLaunchKernelGGL((attend_kernel<D, F, H, W, 4>), grid, dim3(256), 0, stream, g);
   };
   auto with = [&](auto dim, auto fmt) {
     const std::true_type yes{};
@@ -650,7 +717,7 @@ int cache_attend_launch(const Cache& c, const Sequences& s, const AttendArgs& a,
   else
     c.format == CACHE_FP4 ? with(std::integral_constant<int, 128>{}, fp4) : with(std::integral_constant<int, 128>{}, fp8);
   NOISE_CHECK_LAUNCH();
-  if (r.join) {
+  if (r.p.groups) {
     const dim3 grid((unsigned)(s.rows * a.heads));
     auto join = [&](auto dim, auto f16_) {
       hipLaunchKernelGGL((join_kernel<decltype(dim)::value, decltype(f16_)::value>), grid, dim3(256), 0, stream, g);
