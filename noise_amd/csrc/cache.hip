@@ -7,9 +7,11 @@
 // power of two is exact, so the codes are the nearest ones of the input itself. A group with an infinity or a NaN gets byte
 // 255 and reads back as NaN.
 //
-// Both kernels only move bytes. A lane takes 8 channels of one head (16 or 32 bytes of a row, 4 or 8 of codes) and the four
-// lanes of a group share its maximum through DPP; consecutive lanes take consecutive channels, so a wave reads whole rows. A
-// workgroup takes consecutive rows, which fill consecutive bytes of a page.
+// Both kernels only move bytes. A workgroup takes up to 64 consecutive rows of up to 8 heads, of the keys or of the values, and
+// turns them over in LDS: the rows are read or written in their own order (a lane 8 channels, 16 or 32 bytes; the four
+// lanes of a group share its maximum through DPP), the codes in the cache's, head by head, where consecutive tokens of a page
+// are consecutive bytes (a lane 16 bytes). Reading 64 bytes of a head here and there between the stores instead, without LDS, took
+// 24 sequences of up to 8192 tokens, 8 heads of 128 in e2m1, 137 us where their stores alone take 85.
 #include <type_traits>
 
 #include "common.h"
@@ -116,82 +118,158 @@ __device__ __forceinline__ void values8(uint2 codes, float scale, float (&x)[8])
   for (int e = 0; e < 4; ++e) x[2 * e] = p[e].x * scale, x[2 * e + 1] = p[e].y * scale;
 }
 
-constexpr int ROWS_MAX = 16;  // rows of a workgroup
+constexpr int ROWS_MAX = 64;  // rows of a workgroup, at most a wave's lanes
+constexpr long NO_PLACE = -1, BAD_PLACE = -2;
 
-// Slots of the workgroup's rows into `slot`: -1 for a row at no place (no sequence, a negative position), -2 for a page that
-// the cache does not have.
-__device__ __forceinline__ void find_slots(const Cache& c, const Sequences& s, int r0, int nr, long* slot) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (int r = wave; r < nr; r += NTH / 64) {
-    const Place at = place_of(s, r0 + r);
-    long x = -1;
-    if (at.b >= 0 && at.pos >= 0) {
-      x = slot_of(c, s, at.b, at.pos);
-      if (x < 0) x = -2;
+// The code rows (of kv head 0) of the workgroup's rows into `base`, or NO_PLACE, or BAD_PLACE for a page that the cache does not
+// have. A lane a row: the first row's sequence is found by the wave, and most rows are in the same one; the others search on.
+// One wave, whose first thread is t0.
+__device__ __forceinline__ void find_rows(const Cache& c, const Sequences& s, int r0, int nr, long* base, int t0) {
+  const int r = threadIdx.x - t0, i = r0 + min(r, nr - 1);
+  int b = i;
+  long pos = -1;
+  if (s.starts) {
+    b = find_sequence(s.starts, s.n, r0);
+    if (b < s.n && s.starts[b + 1] <= i) {
+      int lo = b + 1, hi = s.n;  // the entries of starts[1 ..] that are <= i: at least lo, at most hi
+      while (lo < hi) {
+        const int mid = lo + (hi - lo + 1) / 2;
+        if (s.starts[mid] <= i)
+          lo = mid;
+        else
+          hi = mid - 1;
+      }
+      b = lo;
     }
-    if ((threadIdx.x & 63) == 0) slot[r] = x;
+    if (b < s.n) {
+      const int s0 = s.starts[b], s1 = s.starts[b + 1];
+      if (i >= s0 && i < s1) pos = (long)s.lengths[b] - s1 + i;
+    }
+  } else {
+    pos = (long)s.lengths[b] - 1;
+  }
+  long x = NO_PLACE;
+  if (pos >= 0) {
+    x = slot_of(c, s, b, pos);
+    const long page = x >> c.page_shift;
+    x = x < 0 ? BAD_PLACE : ((page * c.kv_heads) << c.page_shift) + (x & ((1 << c.page_shift) - 1));
+  }
+  if (r < nr) base[r] = x;
+}
+
+constexpr int HEADS = 8;  // heads of a workgroup at most
+
+// What a workgroup turns over in LDS: codes [head][row + one of padding][ROW bytes], so that the heads of a wave lie in different
+// banks, and scale bytes [head][row][GROUPS].
+template <int FMT, int DIM>
+struct Turn {
+  static constexpr int CH = DIM / 8, GROUPS = DIM / 32, ROW = FMT == CACHE_FP4 ? DIM / 2 : DIM, BYTES = ROW / CH;
+  static __host__ __device__ int code_bytes(int heads, int nr) { return heads * (nr + 1) * ROW; }
+  static __host__ __device__ int bytes(int heads, int nr) { return code_bytes(heads, nr) + heads * nr * GROUPS; }
+};
+
+// body(at, cache byte) for every 16 bytes of codes of the workgroup's rows, in the cache's order: from byte
+// `at` of the LDS area; then scale() likewise for the scale bytes of every row and head.
+template <int FMT, int DIM, class F, class G>
+__device__ __forceinline__ void in_cache_order(const long* base, int page_shift, int h0, int heads, int nr, int log_nr, F body, G scale) {
+  using T = Turn<FMT, DIM>;
+  constexpr int PARTS = T::ROW / 16;
+  const int all = (heads * PARTS) << log_nr;
+  if (threadIdx.x >= NTH) return;
+#pragma unroll 4
+  for (int u = threadIdx.x; u < all; u += NTH) {
+    const int part = u % PARTS, r = (u / PARTS) & ((1 << log_nr) - 1), h = (u / PARTS) >> log_nr;
+    const long at = r < nr ? base[r] : NO_PLACE;
+    if (at >= 0) body((h * ((1 << log_nr) + 1) + r) * T::ROW + 16 * part, (at + ((long)(h0 + h) << page_shift)) * T::ROW + 16 * part);
+  }
+  for (int u = threadIdx.x; u < heads << log_nr; u += NTH) {
+    const int r = u & ((1 << log_nr) - 1), h = u >> log_nr;
+    const long at = r < nr ? base[r] : NO_PLACE;
+    if (at >= 0) scale(u * T::GROUPS, (at + ((long)(h0 + h) << page_shift)) * T::GROUPS);
+  }
+}
+
+// One workgroup: 2^log_nr rows (the last one fewer) of a slab of heads; blockIdx.y even the keys, odd the values. A fifth wave looks
+// the rows' places up (three loads, one after the other) while the others quantise.
+template <int TYPE, int FMT, int DIM>
+__global__ void __launch_bounds__(NTH + 64) cache_write_kernel(Cache c, Sequences s, Heads k, Heads v, int log_nr) {
+  using T = Turn<FMT, DIM>;
+  extern __shared__ __attribute__((aligned(16))) uint8_t turn[];
+  __shared__ long base[ROWS_MAX];
+  const int r0 = blockIdx.x << log_nr, nr = min(1 << log_nr, s.rows - r0);
+  const int h0 = blockIdx.y / 2 * HEADS, heads = min(HEADS, c.kv_heads - h0);
+  uint8_t* turned = turn + T::code_bytes(heads, 1 << log_nr);
+  const Heads in = blockIdx.y & 1 ? v : k;
+  uint8_t *codes = blockIdx.y & 1 ? c.v : c.k, *scales = blockIdx.y & 1 ? c.vs : c.ks;
+  const int per = heads * T::CH, step = NTH / per, first = threadIdx.x / per, x0 = threadIdx.x % per, h = x0 / T::CH, d = x0 % T::CH;
+  const long from = (long)(h0 + h) * in.hs + 8 * d;
+  if (threadIdx.x >= NTH) {
+    find_rows(c, s, r0, nr, base, NTH);
+  } else if (first < step) {
+#pragma unroll 4
+    for (int r = first; r < nr; r += step) {
+      float x[8];
+      load8<TYPE>(in.p, (r0 + r) * in.ld + from, x);
+      uint2 q;
+      const unsigned char e = quantise8<FMT>(x, q);
+      uint8_t* o = turn + (h * ((1 << log_nr) + 1) + r) * T::ROW + d * T::BYTES;
+      if constexpr (FMT == CACHE_FP4)
+        *reinterpret_cast<unsigned*>(o) = q.x;
+      else
+        *reinterpret_cast<uint2*>(o) = q;
+      if (d % 4 == 0) turned[((h << log_nr) + r) * T::GROUPS + d / 4] = e;
+    }
   }
   __syncthreads();
+  in_cache_order<FMT, DIM>(
+      base, c.page_shift, h0, heads, nr, log_nr,
+      [&](int at, long to) { *reinterpret_cast<u32x4*>(codes + to) = *reinterpret_cast<const u32x4*>(turn + at); },
+      [&](int at, long to) {
+        if constexpr (DIM == 64)
+          *reinterpret_cast<uint16_t*>(scales + to) = *reinterpret_cast<const uint16_t*>(turned + at);
+        else
+          *reinterpret_cast<unsigned*>(scales + to) = *reinterpret_cast<const unsigned*>(turned + at);
+      });
 }
 
-// One workgroup: `nr` rows (the last one fewer), blockIdx.y 0 the keys, 1 the values.
-template <int TYPE, int FMT>
-__global__ void __launch_bounds__(NTH) cache_write_kernel(Cache c, Sequences s, Heads k, Heads v, int nr) {
-  __shared__ long slot[ROWS_MAX];
-  const int r0 = blockIdx.x * nr;
-  nr = min(nr, s.rows - r0);
-  find_slots(c, s, r0, nr, slot);
-  const Heads in = blockIdx.y ? v : k;
-  uint8_t *codes = blockIdx.y ? c.v : c.k, *scales = blockIdx.y ? c.vs : c.ks;
-  const int ch = c.dim / 8, per = c.kv_heads * ch;  // chunks of a head, of a row
-  constexpr int BYTES = FMT == CACHE_FP4 ? 4 : 8;
-  for (int i = threadIdx.x; i < nr * per; i += NTH) {
-    const int r = i / per, h = (i % per) / ch, d = i % ch;
-    const long at = slot[r];
-    float x[8];
-    load8<TYPE>(in.p, (r0 + r) * in.ld + h * in.hs + 8 * d, x);
-    uint2 q;
-    const unsigned char e = quantise8<FMT>(x, q);
-    if (at < 0) continue;
-    // token row of this head: page * kv_heads * page size + h * page size + token
-    const long page = at >> c.page_shift, row = ((page * c.kv_heads + h) << c.page_shift) + (at & ((1 << c.page_shift) - 1));
-    uint8_t* o = codes + row * (ch * BYTES) + d * BYTES;
+template <int TYPE, int FMT, int DIM>
+__global__ void __launch_bounds__(NTH) cache_read_kernel(Cache c, Sequences s, void* ko, void* vo, int log_nr) {
+  using T = Turn<FMT, DIM>;
+  extern __shared__ __attribute__((aligned(16))) uint8_t turn[];
+  __shared__ long base[ROWS_MAX];
+  const int r0 = blockIdx.x << log_nr, nr = min(1 << log_nr, s.rows - r0);
+  const int h0 = blockIdx.y / 2 * HEADS, heads = min(HEADS, c.kv_heads - h0);
+  uint8_t* turned = turn + T::code_bytes(heads, 1 << log_nr);
+  if (threadIdx.x < 64) find_rows(c, s, r0, nr, base, 0);
+  __syncthreads();
+  void* out = blockIdx.y & 1 ? vo : ko;
+  const uint8_t *codes = blockIdx.y & 1 ? c.v : c.k, *scales = blockIdx.y & 1 ? c.vs : c.ks;
+  in_cache_order<FMT, DIM>(
+      base, c.page_shift, h0, heads, nr, log_nr,
+      [&](int at, long from) { *reinterpret_cast<u32x4*>(turn + at) = *reinterpret_cast<const u32x4*>(codes + from); },
+      [&](int at, long from) {
+        if constexpr (DIM == 64)
+          *reinterpret_cast<uint16_t*>(turned + at) = *reinterpret_cast<const uint16_t*>(scales + from);
+        else
+          *reinterpret_cast<unsigned*>(turned + at) = *reinterpret_cast<const unsigned*>(scales + from);
+      });
+  __syncthreads();
+  const int per = heads * T::CH, step = NTH / per, first = threadIdx.x / per, x0 = threadIdx.x % per, h = x0 / T::CH, d = x0 % T::CH;
+  if (first >= step) return;
+#pragma unroll 4
+  for (int r = first; r < nr; r += step) {
+    const long at = base[r];
+    const uint8_t* p = turn + (h * ((1 << log_nr) + 1) + r) * T::ROW + d * T::BYTES;
+    uint2 q = make_uint2(0, 0);
     if constexpr (FMT == CACHE_FP4)
-      *reinterpret_cast<unsigned*>(o) = q.x;
+      q.x = *reinterpret_cast<const unsigned*>(p);
     else
-      *reinterpret_cast<uint2*>(o) = q;
-    if (d % 4 == 0) scales[row * (ch / 4) + d / 4] = e;
-  }
-}
-
-template <int TYPE, int FMT>
-__global__ void __launch_bounds__(NTH) cache_read_kernel(Cache c, Sequences s, void* ko, void* vo, int nr) {
-  __shared__ long slot[ROWS_MAX];
-  const int r0 = blockIdx.x * nr;
-  nr = min(nr, s.rows - r0);
-  find_slots(c, s, r0, nr, slot);
-  void* out = blockIdx.y ? vo : ko;
-  const uint8_t *codes = blockIdx.y ? c.v : c.k, *scales = blockIdx.y ? c.vs : c.ks;
-  const int ch = c.dim / 8, per = c.kv_heads * ch;
-  constexpr int BYTES = FMT == CACHE_FP4 ? 4 : 8;
-  for (int i = threadIdx.x; i < nr * per; i += NTH) {
-    const int r = i / per, h = (i % per) / ch, d = i % ch;
-    const long at = slot[r];
+      q = *reinterpret_cast<const uint2*>(p);
+    const unsigned e = turned[((h << log_nr) + r) * T::GROUPS + d / 4];
+    if (at < 0) q = make_uint2(0, 0);  // (what LDS held before)
     float x[8];
-    if (at >= 0) {
-      const long page = at >> c.page_shift, row = ((page * c.kv_heads + h) << c.page_shift) + (at & ((1 << c.page_shift) - 1));
-      const uint8_t* p = codes + row * (ch * BYTES) + d * BYTES;
-      uint2 q = make_uint2(0, 0);
-      if constexpr (FMT == CACHE_FP4)
-        q.x = *reinterpret_cast<const unsigned*>(p);
-      else
-        q = *reinterpret_cast<const uint2*>(p);
-      values8<FMT>(q, scale_of(scales[row * (ch / 4) + d / 4]), x);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = at == -1 ? 0.f : __uint_as_float(0x7fc00000u);
-    }
-    store8<TYPE>(out, ((long)(r0 + r) * per + i % per) * 8, x);
+    values8<FMT>(q, at == BAD_PLACE ? __uint_as_float(0x7fc00000u) : at < 0 ? 0.f : scale_of(e), x);
+    store8<TYPE>(out, ((long)(r0 + r) * c.kv_heads * T::CH + h0 * T::CH + x0) * 8, x);
   }
 }
 
@@ -207,21 +285,32 @@ bool bad_cache(const Cache& c, const Sequences& s) {
 
 namespace {
 
-// Rows of a workgroup: 16 where that still gives every CU several workgroups, fewer for short calls.
-int rows_per_group(const Cache& c, const Sequences& s) {
-  int nr = ROWS_MAX;
-  while (nr > 1 && (s.rows + nr - 1) / nr < 2 * num_cus()) nr /= 2;
-  return nr;
+// Rows of a workgroup, as a power of two: 64 (32 of 128 bytes, so that four workgroups fit a CU's LDS) where that still gives every
+// CU eight workgroups, fewer for short calls, but enough to keep its threads busy.
+int log_rows(const Cache& c, const Sequences& s) {
+  const int per = (c.kv_heads < HEADS ? c.kv_heads : HEADS) * (c.dim / 8);
+  int l = c.dim == 128 && c.format == CACHE_FP8 ? 5 : 6;
+  while (l > 0 && ((s.rows - 1) >> l) + 1 < 4 * num_cus() && (per << (l - 1)) >= NTH) --l;
+  return l;
+}
+dim3 grid_of(const Cache& c, const Sequences& s, int l) {
+  return dim3((unsigned)((s.rows - 1) >> l) + 1, 2u * (unsigned)((c.kv_heads + HEADS - 1) / HEADS));
 }
 
-// launch(type, format) with both as compile-time constants
+// launch(type, format, dim) with all three as compile-time constants
 template <class F>
-void by_type(int type, int format, F launch) {
+void by_type(int type, const Cache& c, F launch) {
   auto of = [&](auto t) {
-    if (format == CACHE_FP4)
-      launch(t, std::integral_constant<int, CACHE_FP4>{});
+    auto with = [&](auto f) {
+      if (c.dim == 64)
+        launch(t, f, std::integral_constant<int, 64>{});
+      else
+        launch(t, f, std::integral_constant<int, 128>{});
+    };
+    if (c.format == CACHE_FP4)
+      with(std::integral_constant<int, CACHE_FP4>{});
     else
-      launch(t, std::integral_constant<int, CACHE_FP8>{});
+      with(std::integral_constant<int, CACHE_FP8>{});
   };
   if (type == ROWS_BF16)
     of(std::integral_constant<int, ROWS_BF16>{});
@@ -238,10 +327,11 @@ int cache_write_launch(const Cache& c, const Sequences& s, const Heads& k, const
   const int unit = type == ROWS_F32 ? 4 : 8;  // elements of a 16-byte load
   for (const Heads* h : {&k, &v})
     if (!h->p || ((uintptr_t)h->p & 15) || h->ld % unit || h->hs % unit || h->ld < 0 || h->hs < 0) return NOISE_EINVAL;
-  const int nr = rows_per_group(c, s);
-  const dim3 grid((unsigned)((s.rows + nr - 1) / nr), 2);
-  by_type(type, c.format, [&](auto t, auto f) {
-    hipLaunchKernelGGL((cache_write_kernel<decltype(t)::value, decltype(f)::value>), grid, dim3(NTH), 0, stream, c, s, k, v, nr);
+  const int l = log_rows(c, s), heads = c.kv_heads < HEADS ? c.kv_heads : HEADS;
+  by_type(type, c, [&](auto t, auto f, auto d) {
+    constexpr int TY = decltype(t)::value, F = decltype(f)::value, D = decltype(d)::value;
+    const int lds = Turn<F, D>::bytes(heads, 1 << l);
+    hipLaunchKernelGGL((cache_write_kernel<TY, F, D>), grid_of(c, s, l), dim3(NTH + 64), lds, stream, c, s, k, v, l);
   });
   NOISE_CHECK_LAUNCH();
   return NOISE_OK;
@@ -250,10 +340,11 @@ int cache_write_launch(const Cache& c, const Sequences& s, const Heads& k, const
 int cache_read_launch(const Cache& c, const Sequences& s, void* k, void* v, int type, hipStream_t stream) {
   if (bad_cache(c, s) || type < ROWS_BF16 || type > ROWS_F32 || !k || !v || (((uintptr_t)k | (uintptr_t)v) & 15))
     return NOISE_EINVAL;
-  const int nr = rows_per_group(c, s);
-  const dim3 grid((unsigned)((s.rows + nr - 1) / nr), 2);
-  by_type(type, c.format, [&](auto t, auto f) {
-    hipLaunchKernelGGL((cache_read_kernel<decltype(t)::value, decltype(f)::value>), grid, dim3(NTH), 0, stream, c, s, k, v, nr);
+  const int l = log_rows(c, s), heads = c.kv_heads < HEADS ? c.kv_heads : HEADS;
+  by_type(type, c, [&](auto t, auto f, auto d) {
+    constexpr int TY = decltype(t)::value, F = decltype(f)::value, D = decltype(d)::value;
+    const int lds = Turn<F, D>::bytes(heads, 1 << l);
+    hipLaunchKernelGGL((cache_read_kernel<TY, F, D>), grid_of(c, s, l), dim3(NTH), lds, stream, c, s, k, v, l);
   });
   NOISE_CHECK_LAUNCH();
   return NOISE_OK;

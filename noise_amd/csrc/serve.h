@@ -84,19 +84,6 @@ __device__ __forceinline__ int find_sequence(const int* starts, int n, int i) {
   return lo + __builtin_popcountll(m);
 }
 
-// Row i's sequence and position; position -1 and b = -1 for a row of no sequence.
-struct Place {
-  int b;
-  long pos;
-};
-__device__ __forceinline__ Place place_of(const Sequences& s, int i) {
-  if (!s.starts) return i < s.n ? Place{i, (long)s.lengths[i] - 1} : Place{-1, -1};
-  const int b = __builtin_amdgcn_readfirstlane(find_sequence(s.starts, s.n, i));
-  if (b >= s.n) return Place{-1, -1};
-  const int s0 = s.starts[b], s1 = s.starts[b + 1];
-  if (i < s0 || i >= s1) return Place{-1, -1};
-  return Place{b, (long)s.lengths[b] - s1 + i};
-}
 // The slot (page * page size + token) of a position, or -1 where the table names no page of the cache for it.
 __device__ __forceinline__ long slot_of(const Cache& c, const Sequences& s, int b, long pos) {
   const long pg = pos >> c.page_shift;
