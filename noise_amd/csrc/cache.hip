@@ -7,7 +7,7 @@
 // power of two is exact, so the codes are the nearest ones of the input itself. A group with an infinity or a NaN gets byte
 // 255 and reads back as NaN.
 //
-// Both kernels only move bytes. A workgroup takes up to 64 consecutive rows of up to 8 heads, of the keys or of the values, and
+// Both kernels only move bytes. A workgroup takes up to 16 consecutive rows of up to 8 heads, of the keys or of the values, and
 // turns them over in LDS: the rows are read or written in their own order (a lane 8 channels, 16 or 32 bytes; the four
 // lanes of a group share its maximum through DPP), the codes in the cache's, head by head, where consecutive tokens of a page
 // are consecutive bytes (a lane 16 bytes). Reading 64 bytes of a head here and there between the stores instead, without LDS, took
@@ -118,7 +118,7 @@ __device__ __forceinline__ void values8(uint2 codes, float scale, float (&x)[8])
   for (int e = 0; e < 4; ++e) x[2 * e] = p[e].x * scale, x[2 * e + 1] = p[e].y * scale;
 }
 
-constexpr int ROWS_MAX = 64;  // rows of a workgroup, at most a wave's lanes
+constexpr int ROWS_MAX = 16;  // rows of a workgroup, at most a wave's lanes
 constexpr long NO_PLACE = -1, BAD_PLACE = -2;
 
 // The code rows (of kv head 0) of the workgroup's rows into `base`, or NO_PLACE, or BAD_PLACE for a page that the cache does not
@@ -285,11 +285,11 @@ bool bad_cache(const Cache& c, const Sequences& s) {
 
 namespace {
 
-// Rows of a workgroup, as a power of two: 64 (32 of 128 bytes, so that four workgroups fit a CU's LDS) where that still gives every
-// CU eight workgroups, fewer for short calls, but enough to keep its threads busy.
+// Rows of a workgroup, as a power of two: 16, fewer for short calls, but enough to keep its threads busy. (The read of the comment
+// at the top: 16 rows 111 us, 32 115, 64 121: more workgroups that read and write at the same time.)
 int log_rows(const Cache& c, const Sequences& s) {
   const int per = (c.kv_heads < HEADS ? c.kv_heads : HEADS) * (c.dim / 8);
-  int l = c.dim == 128 && c.format == CACHE_FP8 ? 5 : 6;
+  int l = 4;
   while (l > 0 && ((s.rows - 1) >> l) + 1 < 4 * num_cus() && (per << (l - 1)) >= NTH) --l;
   return l;
 }
