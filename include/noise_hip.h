@@ -564,7 +564,8 @@ int noise_cache_read(const noise_cache_t* cache, const noise_sequences_t* seqs, 
 /* y = softmax(scale q K^T) V [rows, heads, dim] of the rows' queries q over the cached keys and values of their sequences. NaN
  * for a row that sees a bad place; zero or left as it was (fill) for a row of no sequence. Workspace (16-byte aligned):
  * noise_cache_attend_workspace_size(), a function of the structs' numbers and of whether starts is null. */
-int noise_cache_attend_workspace_size(const noise_cache_t* cache, const noise_sequences_t* seqs, int heads, size_t* bytes);
+int noise_cache_attend_workspace_size(const noise_cache_t* cache, const noise_sequences_t* seqs, int heads, int type,
+                                      size_t* bytes);
 int noise_cache_attend(const noise_cache_t* cache, const noise_sequences_t* seqs, const void* q, long q_ld, long q_hs, int type,
                        int heads, int window, int sinks, float scale, void* y, int fill, void* workspace,
                        size_t workspace_bytes, noise_stream_t stream);

@@ -72,7 +72,7 @@ SIGNATURES = {
     'noise_sink_attention': [P, L, L, P, L, L, P, L, L, P, I, I, I, I, I, I, I, I, I, F, P, I, P],
     'noise_cache_write': [P, P, P, L, L, P, L, L, I, P],
     'noise_cache_read': [P, P, P, P, I, P],
-    'noise_cache_attend_workspace_size': [P, P, I, SP],
+    'noise_cache_attend_workspace_size': [P, P, I, I, SP],
     'noise_cache_attend': [P, P, P, L, L, I, I, I, I, F, P, I, P, S, P],
 }
 

@@ -138,12 +138,13 @@ class KVCache:
         heads = q.shape[1]
         q, qp, ql, qh = heads_rows(q)
         call = ctypes.addressof(seqs)
-        shape = (seqs.sequences, seqs.rows, seqs.table_pages, starts is None, heads)
+        shape = (seqs.sequences, seqs.rows, seqs.table_pages, starts is None, heads, q.dtype)
         size = self._sizes.get(shape)
         if size is None:
             if len(self._sizes) >= 256:
                 self._sizes.clear()
-            size = self._sizes[shape] = _lib.size_query('noise_cache_attend_workspace_size', self._ptr, call, heads)
+            size = self._sizes[shape] = _lib.size_query('noise_cache_attend_workspace_size', self._ptr, call, heads,
+                                                            ROW_TYPES[q.dtype])
         ws = torch.empty(size, device=self.device, dtype=torch.uint8) if size else None
         launch(self.device, 'noise_cache_attend', self._ptr, call, qp, ql, qh, ROW_TYPES[q.dtype], heads, window, sinks, scale,
                y.data_ptr(), fill, _ptr(ws), size)

@@ -713,12 +713,14 @@ int noise_cache_read(const noise_cache_t* cache, const noise_sequences_t* seqs, 
   return cache_read_launch(c, s, k, v, type, static_cast<hipStream_t>(stream));
 }
 
-int noise_cache_attend_workspace_size(const noise_cache_t* cache, const noise_sequences_t* seqs, int heads, size_t* bytes) {
+int noise_cache_attend_workspace_size(const noise_cache_t* cache, const noise_sequences_t* seqs, int heads, int type,
+                                      size_t* bytes) {
   Cache c;
   Sequences s;
   if (!bytes || !copy_cache(cache, seqs, &c, &s)) return NOISE_EINVAL;
   AttendArgs a{};
   a.heads = heads;
+  a.type = type;
   return cache_attend_workspace(c, s, a, bytes);
 }
 

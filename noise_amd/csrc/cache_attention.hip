@@ -202,9 +202,15 @@ struct Args {
   float2* ml;       // [groups, 2, RT] under these maxima, with these sums of probabilities
 };
 
+// Workgroups on a CU: three, or two where a third's registers would spill (a reload waits for all loads on their way; 16 sequences of
+// 16384 tokens, fp16 queries over e4m3: 70 us with three, 54 with two; over e2m1 of dim 64 three 63 us, two 75).
+constexpr int resident(int dim, int format, bool f16) {
+  return (format == CACHE_FP8 && (f16 || dim == 128)) || (f16 && dim == 128) ? 2 : 3;
+}
+
 // WIDE: pages hold whole blocks. F16: fp16 queries (two bf16 terms). NW waves.
 template <int DIM, int FMT, bool F16, bool WIDE, int NW>
-__global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : 3) attend_kernel(Args g) {
+__global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : resident(DIM, FMT, F16)) attend_kernel(Args g) {
   using G = Geo<DIM, FMT>;
   constexpr int BK = G::BK, KT = G::KT, KC = G::KC, DT = G::DT, QS = G::QS, KW = G::KW, VW = G::VW, VN = G::VN;
   constexpr int SHIFT = DIM == 64 ? 6 : 5;
@@ -629,7 +635,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args g) {
 }
 
 bool bad_attend(const Cache& c, const Sequences& s, const AttendArgs& a) {
-  return bad_cache(c, s) || a.heads <= 0 || a.heads > 1024 || a.heads % c.kv_heads || a.window < 0 || a.sinks < 0;
+  return bad_cache(c, s) || (a.type != ROWS_BF16 && a.type != ROWS_F16) || a.heads <= 0 || a.heads > 1024 || a.heads % c.kv_heads || a.window < 0 || a.sinks < 0;
 }
 
 // How a call is cut, by upper bounds of what the GPU finds from the lengths.
@@ -647,7 +653,7 @@ Shape shape_of(const Cache& c, const Sequences& s, const AttendArgs& a) {
   // by alignment)
   const long full = (long)s.rows * r.p.group / RT;
   const long tiles = (s.starts ? full + (s.n < s.rows ? s.n : s.rows) : (long)s.rows * ((r.p.group + RT - 1) / RT)) * c.kv_heads;
-  const long blocks = (r.p.cap >> r.p.block_shift) + 2, fill = 3l * num_cus();
+  const long blocks = (r.p.cap >> r.p.block_shift) + 2, fill = (long)resident(c.dim, c.format, a.type == ROWS_F16) * num_cus();
   // A workgroup a tile, and no second kernel, where a table names so few keys that this costs no more than sharing them out (a
   // round takes about 1.4 us): 11 blocks of 8 heads on eight waves 8.2 us, shared 7.3 + 4.4; 64 sequences of 33 blocks 20.8,
   // shared 23.8 + 4.8; but one of 63 blocks 17.5, shared 7.3 + 5.7. Also where there are many tiles, or more rounds than fit.
@@ -676,8 +682,7 @@ int cache_attend_workspace(const Cache& c, const Sequences& s, const AttendArgs&
 
 int cache_attend_launch(const Cache& c, const Sequences& s, const AttendArgs& a, void* ws, size_t ws_bytes,
                         hipStream_t stream) {
-  if (bad_attend(c, s, a) || bad_heads(a.q) || !a.y || ((uintptr_t)a.y & 15) || (a.type != ROWS_BF16 && a.type != ROWS_F16) ||
-      !(a.scale >= 0.f) || a.scale > 3.4e38f)
+  if (bad_attend(c, s, a) || bad_heads(a.q) || !a.y || ((uintptr_t)a.y & 15) || !(a.scale >= 0.f) || a.scale > 3.4e38f)
     return NOISE_EINVAL;
   const Shape r = shape_of(c, s, a);
   size_t need = 0;

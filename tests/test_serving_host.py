@@ -40,7 +40,7 @@ def test_bad_caches_and_rows_are_refused(c, s):
     assert lib.noise_cache_write(a, b, 16, 512, 64, 16, 512, 64, 0, None) == EINVAL
     assert lib.noise_cache_read(a, b, 16, 16, 0, None) == EINVAL
     assert lib.noise_cache_attend(a, b, 16, 512, 64, 0, 8, 100, 0, 0.125, 16, 1, 16, 1 << 40, None) == EINVAL
-    assert lib.noise_cache_attend_workspace_size(a, b, 8, ctypes.byref(ctypes.c_size_t())) == EINVAL
+    assert lib.noise_cache_attend_workspace_size(a, b, 8, 0, ctypes.byref(ctypes.c_size_t())) == EINVAL
 
 
 def test_bad_operands_are_refused():
