@@ -202,15 +202,17 @@ struct Args {
   float2* ml;       // [groups, 2, RT] under these maxima, with these sums of probabilities
 };
 
-// Workgroups on a CU: three, or two where a third's registers would spill (a reload waits for all loads on their way; 16 sequences of
-// 16384 tokens, fp16 queries over e4m3: 70 us with three, 54 with two; over e2m1 of dim 64 three 63 us, two 75).
-constexpr int resident(int dim, int format, bool f16) {
-  return (format == CACHE_FP8 && (f16 || dim == 128)) || (f16 && dim == 128) ? 2 : 3;
+// Workgroups on a CU. e4m3: two, whose blocks on their way are as many bytes as e2m1's three (16 sequences of 16384 tokens, fp16
+// queries, dim 64: 54 us, with three 59; dim 128 54 and 60); e2m1: three (48 sequences of up to 32768 tokens 93 us; two 101, four
+// 95), or two where a third's registers would spill: a reload waits for all loads on their way.
+constexpr int resident(int dim, int format, bool f16, bool many) {
+  return format == CACHE_FP8 || (many && f16 && dim == 128) ? 2 : 3;
 }
 
-// WIDE: pages hold whole blocks. F16: fp16 queries (two bf16 terms). NW waves.
-template <int DIM, int FMT, bool F16, bool WIDE, int NW>
-__global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : resident(DIM, FMT, F16)) attend_kernel(Args g) {
+// WIDE: pages hold whole blocks. F16: fp16 queries (two bf16 terms). MANY: rows of a tile may lie at different positions (with one row
+// a sequence, whatever one row sees all see, and what none sees is zero before it is multiplied). NW waves.
+template <int DIM, int FMT, bool F16, bool WIDE, bool MANY, int NW>
+__global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : resident(DIM, FMT, F16, MANY)) attend_kernel(Args g) {
   using G = Geo<DIM, FMT>;
   constexpr int BK = G::BK, KT = G::KT, KC = G::KC, DT = G::DT, QS = G::QS, KW = G::KW, VW = G::VW, VN = G::VN;
   constexpr int SHIFT = DIM == 64 ? 6 : 5;
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : resident(DIM, FMT, F16)
       for (int x = 0; x < 4; ++x) {
         const u32x4 val = bf16_of<FMT>(&r.v[n][x * (VW / 4)], vs);
         *reinterpret_cast<u32x4*>(dst + ((vwr ^ (32 * (x >> 1))) + 16 * (x & 1))) = val;
-        if (!whole)
+        if (MANY && !whole)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             odd |= ((val[e] & 0x7f80u) == 0x7f80u) | ((val[e] & 0x7f800000u) == 0x7f800000u);
@@ -474,7 +476,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : resident(DIM, FMT, F16)
       const bf16x4 lo = __builtin_bit_cast(bf16x4, part[0]), hi = __builtin_bit_cast(bf16x4, part[1]);
       return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
-    if (!__any(odd)) {
+    if (!MANY || !__any(odd)) {
 #pragma unroll
       for (int h = 0; h < KC; ++h)
 #pragma unroll
@@ -653,7 +655,7 @@ Shape shape_of(const Cache& c, const Sequences& s, const AttendArgs& a) {
   // by alignment)
   const long full = (long)s.rows * r.p.group / RT;
   const long tiles = (s.starts ? full + (s.n < s.rows ? s.n : s.rows) : (long)s.rows * ((r.p.group + RT - 1) / RT)) * c.kv_heads;
-  const long blocks = (r.p.cap >> r.p.block_shift) + 2, fill = (long)resident(c.dim, c.format, a.type == ROWS_F16) * num_cus();
+  const long blocks = (r.p.cap >> r.p.block_shift) + 2, fill = (long)resident(c.dim, c.format, a.type == ROWS_F16, s.starts) * num_cus();
   // A workgroup a tile, and no second kernel, where a table names so few keys that this costs no more than sharing them out (a
   // round takes about 1.4 us): 11 blocks of 8 heads on eight waves 8.2 us, shared 7.3 + 4.4; 64 sequences of 33 blocks 20.8,
   // shared 23.8 + 4.8; but one of 63 blocks 17.5, shared 7.3 + 5.7. Also where there are many tiles, or more rounds than fit.
@@ -698,22 +700,23 @@ int cache_attend_launch(const Cache& c, const Sequences& s, const AttendArgs& a,
   g.part = static_cast<float*>(ws);
   g.ml = ws ? reinterpret_cast<float2*>(static_cast<char*>(ws) + part_bytes(c, r)) : nullptr;
   const bool wide = (1 << c.page_shift) >= (1 << r.p.block_shift);
-  auto launch = [&](auto dim, auto fmt, auto f16_, auto wide_) {
+  auto launch = [&](auto dim, auto fmt, auto f16_, auto wide_, auto many) {
     constexpr int D = decltype(dim)::value, F = decltype(fmt)::value;
-    constexpr bool H = decltype(f16_)::value, W = decltype(wide_)::value;
+    constexpr bool H = decltype(f16_)::value, W = decltype(wide_)::value, M = decltype(many)::value;
     const dim3 grid((unsigned)(g.items + g.fills));
     if (r.p.waves == 8)
-      hipLaunchKernelGGL((attend_kernel<D, F, H, W, 8>), grid, dim3(512), 0, stream, g);
+      hipLaunchKernelGGL((attend_kernel<D, F, H, W, M, 8>), grid, dim3(512), 0, stream, g);
     else
-      hipLaunchKernelGGL((attend_kernel<D, F, H, W, 4>), grid, dim3(256), 0, stream, g);
+      hipLaunchKernelGGL((attend_kernel<D, F, H, W, M, 4>), grid, dim3(256), 0, stream, g);
   };
   auto with = [&](auto dim, auto fmt) {
     const std::true_type yes{};
     const std::false_type no{};
+    auto of = [&](auto f16_, auto wide_) { s.starts ? launch(dim, fmt, f16_, wide_, yes) : launch(dim, fmt, f16_, wide_, no); };
     if (a.type == ROWS_F16)
-      wide ? launch(dim, fmt, yes, yes) : launch(dim, fmt, yes, no);
+      wide ? of(yes, yes) : of(yes, no);
     else
-      wide ? launch(dim, fmt, no, yes) : launch(dim, fmt, no, no);
+      wide ? of(no, yes) : of(no, no);
   };
   const std::integral_constant<int, CACHE_FP4> fp4{};
   const std::integral_constant<int, CACHE_FP8> fp8{};
