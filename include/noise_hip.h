@@ -510,7 +510,8 @@ int noise_adam_batch(const noise_adam_tensor_t* tensors, int n, float beta1, flo
 /* ---------------------------------------------------------------- serving: prompts, and a key / value cache
  * No counterpart in the reference, which trains and scores; this is what answering with a trained model needs next to
  * it. Rows are packed: `rows` rows of `sequences` sequences, sequence b owning rows starts[b] .. starts[b + 1] (int32,
- * [sequences + 1], nondecreasing; rows outside starts[0] .. starts[sequences] belong to none). A query at position s sees key
+ * [sequences + 1], nondecreasing: where they decrease, rows are left unwritten; rows outside starts[0] .. starts[sequences]
+ * belong to none). A query at position s sees key
  * j when 0 <= j <= s and (s - j <= window or j < sinks); pass INT_MAX for no window. A row that sees no key is zero; keys and
  * values that a row does not see take no part in it, whatever they hold. dim is 64 or 128, heads a multiple of kv_heads,
  * query head h reading kv head h / (heads / kv_heads). */
@@ -541,7 +542,8 @@ typedef struct noise_cache {
 /* The rows of a call: the m rows of sequence b sit at positions lengths[b] - m .. lengths[b] - 1 (the newest tokens of a
  * sequence that holds lengths[b]); starts null: one row a sequence. Position p of sequence b is token p % page_size of
  * page table[b * table_ld + p / page_size] (int32, table_pages entries a sequence). Rows of no sequence and rows at negative
- * positions are at no place; a page outside [0, pages), or a position past the table, is a bad place. */
+ * positions are at no place; a page outside [0, pages), or a position past the table (or from 2^31 - 256 on), is a bad
+ * place. Rows of the table may overlap (table_ld 0: all sequences read one). */
 typedef struct noise_sequences {
   const int* table;
   long table_ld;

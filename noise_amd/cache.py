@@ -6,7 +6,7 @@ one byte, the codes are e2m1 ('fp4', 4.25 bits a channel) or e4m3 ('fp8', 8.25 b
 
 A call names its rows by three int32 tensors on the GPU: `table` [sequences, pages of a sequence], the page of each position of
 each sequence; `lengths` [sequences], the tokens that each sequence holds, the call's own included; `starts` [sequences + 1],
-the rows of each sequence in the packed tensors (None: one row each). The m rows of sequence b sit at its newest positions,
+the rows of each sequence in the packed tensors, nondecreasing (None: one row each). The m rows of sequence b sit at its newest positions,
 lengths[b] - m .. lengths[b] - 1. One decoding step is
 
     lengths += 1
@@ -76,7 +76,7 @@ class KVCache:
                 raise ValueError(f'{rows} rows of {n} sequences need starts')
         elif sequence_starts(starts, self.device) != n:
             raise ValueError(f'starts must have {n + 1} entries')
-        return _lib.Sequences(table.data_ptr(), max(table.stride(0), pages), pages, lengths.data_ptr(), _ptr(starts), n, rows)
+        return _lib.Sequences(table.data_ptr(), table.stride(0) if n > 1 else 0, pages, lengths.data_ptr(), _ptr(starts), n, rows)
 
     def write(self, k, v, table, lengths, starts=None):
         """Quantises the rows k and v [n, kv_heads, dim] (bf16, fp16 or fp32, any strides) into their places. The places of one

@@ -280,7 +280,7 @@ bool bad_cache(const Cache& c, const Sequences& s) {
          c.kv_heads <= 0 || c.kv_heads > 1024 || (c.dim != 64 && c.dim != 128) ||
          (c.format != CACHE_FP4 && c.format != CACHE_FP8) || (((uintptr_t)c.k | (uintptr_t)c.v) & 15) ||
          (((uintptr_t)c.ks | (uintptr_t)c.vs) & 3) || s.n <= 0 || s.rows <= 0 || !s.lengths || s.table_pages < 0 ||
-         (s.table_pages > 0 && (!s.table || s.table_ld < s.table_pages)) || (!s.starts && s.rows != s.n);
+         (s.table_pages > 0 && (!s.table || s.table_ld < 0)) || (!s.starts && s.rows != s.n);
 }
 
 namespace {

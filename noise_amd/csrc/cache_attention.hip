@@ -64,6 +64,7 @@ __device__ __forceinline__ u32x4 bf16_of(const unsigned* w, float scale) {
 // One sequence's share of a call, as the kernels cut it.
 struct Cut {
   int m, len, blocks, tiles;  // rows, tokens, key blocks of its longest tile, tiles of RT rows
+  bool bad;                   // starts that decrease (the counts below would be of more rows than there are)
 };
 struct Plan {
   int group;        // query heads of a kv head
@@ -88,13 +89,15 @@ __device__ __forceinline__ Range range_of(int p0, int p1, int window, int sinks,
 }
 
 __device__ __forceinline__ Cut cut_of(const Sequences& s, const Plan& p, int window, int sinks, int b, int& s0) {
-  Cut c{0, 0, 0, 0};
+  Cut c{0, 0, 0, 0, false};
   s0 = 0;
   if (b >= s.n) return c;
   int s1;
   if (s.starts) {
     s0 = min(max(s.starts[b], 0), s.rows);
-    s1 = min(max(s.starts[b + 1], s0), s.rows);
+    s1 = min(max(s.starts[b + 1], 0), s.rows);
+    c.bad = s1 < s0;
+    if (c.bad) return c;
   } else {
     s0 = b;
     s1 = b + 1;
@@ -133,10 +136,12 @@ __device__ __forceinline__ int rounds_of(const Plan& p, const Cut& c) { return m
 __device__ Line line_of(const Sequences& s, const Plan& p, int kv_heads, int window, int sinks, Kept& kept) {
   const int lane = threadIdx.x & 63;
   int total = 0;
+  bool bad = false;
   for (int b0 = 0; b0 < s.n; b0 += 64) {
     int s0;
     const Cut c = cut_of(s, p, window, sinks, b0 + lane, s0);
     total += c.tiles * rounds_of(p, c);
+    bad |= c.bad;
     if (s.n <= 64) {
       kept.s0[lane] = s0;
       kept.m[lane] = c.m;
@@ -146,7 +151,7 @@ __device__ Line line_of(const Sequences& s, const Plan& p, int kv_heads, int win
     }
   }
   for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
-  total = uniform(total);
+  total = __any(bad) ? 0 : uniform(total);
   return Line{total, (total * kv_heads + p.groups - 1) / p.groups};
 }
 
@@ -160,9 +165,10 @@ __device__ Work find_work(const Sequences& s, const Plan& p, int window, int sin
     Cut c;
     if (p.groups && s.n <= 64) {
       s0 = kept.s0[lane];
-      c = Cut{kept.m[lane], kept.len[lane], kept.blocks[lane], kept.tiles[lane]};
+      c = Cut{kept.m[lane], kept.len[lane], kept.blocks[lane], kept.tiles[lane], false};
     } else {
       c = cut_of(s, p, window, sinks, b0 + lane, s0);
+      if (__any(c.bad)) return w;
     }
     const int each = p.groups ? rounds_of(p, c) : 1;
     const int mine = c.tiles * each;
@@ -205,14 +211,14 @@ struct Args {
 // Workgroups on a CU. e4m3: two, whose blocks on their way are as many bytes as e2m1's three (16 sequences of 16384 tokens, fp16
 // queries, dim 64: 54 us, with three 59; dim 128 54 and 60); e2m1: three (48 sequences of up to 32768 tokens 93 us; two 101, four
 // 95), or two where a third's registers would spill: a reload waits for all loads on their way.
-constexpr int resident(int dim, int format, bool f16, bool many) {
-  return format == CACHE_FP8 || (many && f16 && dim == 128) ? 2 : 3;
+constexpr int resident(int dim, int format, bool f16, bool wide, bool many) {
+  return format == CACHE_FP8 || (many && (!wide || (f16 && dim == 128))) ? 2 : 3;
 }
 
 // WIDE: pages hold whole blocks. F16: fp16 queries (two bf16 terms). MANY: rows of a tile may lie at different positions (with one row
 // a sequence, whatever one row sees all see, and what none sees is zero before it is multiplied). NW waves.
 template <int DIM, int FMT, bool F16, bool WIDE, bool MANY, int NW>
-__global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : resident(DIM, FMT, F16, MANY)) attend_kernel(Args g) {
+__global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : resident(DIM, FMT, F16, WIDE, MANY)) attend_kernel(Args g) {
   using G = Geo<DIM, FMT>;
   constexpr int BK = G::BK, KT = G::KT, KC = G::KC, DT = G::DT, QS = G::QS, KW = G::KW, VW = G::VW, VN = G::VN;
   constexpr int SHIFT = DIM == 64 ? 6 : 5;
@@ -592,16 +598,16 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : resident(DIM, FMT, F16,
 }
 
 // y of the rows whose tile several workgroups share: one workgroup a row and head, its waves taking the others' sums in turn.
-template <int DIM, bool F16>
-__global__ void __launch_bounds__(256) join_kernel(Args g) {
-  constexpr int NW = 4, PER = DIM / 64;
+template <int DIM, bool F16, int NW>
+__global__ void __launch_bounds__(64 * NW) join_kernel(Args g) {
+  constexpr int PER = DIM / 64;
   __shared__ float so[NW][DIM], sl[NW];
   __shared__ Kept kept;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x / g.a.heads, h = blockIdx.x % g.a.heads, kh = h / g.p.group;
   const Line line = line_of(g.s, g.p, g.c.kv_heads, g.a.window, g.a.sinks, kept);
   const Work w = find_work(g.s, g.p, g.a.window, g.a.sinks, 0, row, h % g.p.group, kept);
-  if (!w.found) return;
+  if (!w.found || !line.units) return;
   const int from = kh * line.units + w.at, first = from / line.share, last = (from + w.rounds - 1) / line.share;
   if (first == last) return;
   const int n = last - first + 1, r = ((row - w.s0) * g.p.group + h % g.p.group) % RT;
@@ -625,7 +631,9 @@ __global__ void __launch_bounds__(256) join_kernel(Args g) {
   __syncthreads();
   if (threadIdx.x < DIM) {
     const int d = threadIdx.x;
-    const float l = (sl[0] + sl[1]) + (sl[2] + sl[3]), v = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
+    float l = 0.f, v = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) l += sl[x], v += so[x][d];
     const bool past = w.len - w.m + (row - w.s0) >= g.p.cap;
     const float y = past ? __uint_as_float(0x7fc00000u) : l == 0.f ? 0.f : v / l;
     const long dst = (long)blockIdx.x * DIM + d;
@@ -640,6 +648,9 @@ bool bad_attend(const Cache& c, const Sequences& s, const AttendArgs& a) {
   return bad_cache(c, s) || (a.type != ROWS_BF16 && a.type != ROWS_F16) || a.heads <= 0 || a.heads > 1024 || a.heads % c.kv_heads || a.window < 0 || a.sinks < 0;
 }
 
+// Whether pages hold whole blocks.
+bool wide_pages(const Cache& c) { return (1 << c.page_shift) >= 4096 / c.dim; }
+
 // How a call is cut, by upper bounds of what the GPU finds from the lengths.
 struct Shape {
   Plan p;
@@ -650,12 +661,12 @@ Shape shape_of(const Cache& c, const Sequences& s, const AttendArgs& a) {
   r.p.group = a.heads / c.kv_heads;
   r.p.block_shift = c.dim == 64 ? 6 : 5;
   const long cap = (long)s.table_pages << c.page_shift;
-  r.p.cap = (int)(cap < 0x7fffffffL ? cap : 0x7fffffffL);
+  r.p.cap = (int)(cap < 0x7fffff00L ? cap : 0x7fffff00L);
   // tiles: at most one begun by every sequence beside the full ones; no tile sees more blocks than the table names (and one more
   // by alignment)
   const long full = (long)s.rows * r.p.group / RT;
   const long tiles = (s.starts ? full + (s.n < s.rows ? s.n : s.rows) : (long)s.rows * ((r.p.group + RT - 1) / RT)) * c.kv_heads;
-  const long blocks = (r.p.cap >> r.p.block_shift) + 2, fill = (long)resident(c.dim, c.format, a.type == ROWS_F16, s.starts) * num_cus();
+  const long blocks = (r.p.cap >> r.p.block_shift) + 2, fill = (long)resident(c.dim, c.format, a.type == ROWS_F16, wide_pages(c), s.starts) * num_cus();
   // A workgroup a tile, and no second kernel, where a table names so few keys that this costs no more than sharing them out (a
   // round takes about 1.4 us): 11 blocks of 8 heads on eight waves 8.2 us, shared 7.3 + 4.4; 64 sequences of 33 blocks 20.8,
   // shared 23.8 + 4.8; but one of 63 blocks 17.5, shared 7.3 + 5.7. Also where there are many tiles, or more rounds than fit.
@@ -699,7 +710,7 @@ int cache_attend_launch(const Cache& c, const Sequences& s, const AttendArgs& a,
   g.items = (int)r.items;
   g.part = static_cast<float*>(ws);
   g.ml = ws ? reinterpret_cast<float2*>(static_cast<char*>(ws) + part_bytes(c, r)) : nullptr;
-  const bool wide = (1 << c.page_shift) >= (1 << r.p.block_shift);
+  const bool wide = wide_pages(c);
   auto launch = [&](auto dim, auto fmt, auto f16_, auto wide_, auto many) {
     constexpr int D = decltype(dim)::value, F = decltype(fmt)::value;
     constexpr bool H = decltype(f16_)::value, W = decltype(wide_)::value, M = decltype(many)::value;
@@ -727,8 +738,14 @@ int cache_attend_launch(const Cache& c, const Sequences& s, const AttendArgs& a,
   NOISE_CHECK_LAUNCH();
   if (r.p.groups) {
     const dim3 grid((unsigned)(s.rows * a.heads));
+    // sixteen waves where few rows have many parts (8 rows of 64 parts 8.1 us with four, 6.5 with sixteen), four where rows fill the GPU
     auto join = [&](auto dim, auto f16_) {
-      hipLaunchKernelGGL((join_kernel<decltype(dim)::value, decltype(f16_)::value>), grid, dim3(256), 0, stream, g);
+      constexpr int D = decltype(dim)::value;
+      constexpr bool H = decltype(f16_)::value;
+      if (grid.x <= (unsigned)num_cus())
+        hipLaunchKernelGGL((join_kernel<D, H, 16>), grid, dim3(1024), 0, stream, g);
+      else
+        hipLaunchKernelGGL((join_kernel<D, H, 4>), grid, dim3(256), 0, stream, g);
     };
     const std::integral_constant<int, 64> d64{};
     const std::integral_constant<int, 128> d128{};

@@ -73,22 +73,23 @@ __device__ Tile find_tile(const SinkArgs& a, int id) {
   const bool even = a.heads % 8 == 0;
   const int per = even ? a.heads / 8 : a.heads;  // heads that an index runs over
   Tile t{};
+  // rows of sequence b, negative where starts decrease (then nothing more is found)
   auto rows_of = [&](int b, int& s0) {
     s0 = 0;
     if (b >= a.n) return 0;
-    if (!a.starts) {
-      s0 = b * a.T;
-      return a.T;
-    }
     s0 = min(max(a.starts[b], 0), a.rows);
-    return min(max(a.starts[b + 1], s0), a.rows) - s0;
+    return min(max(a.starts[b + 1], 0), a.rows) - s0;
   };
   // (all counts are below the grid's size)
   int at = j;
   if (!even) {
     int total = 0, s0;
     if (a.starts) {
-      for (int b0 = 0; b0 < a.n; b0 += 64) total += (rows_of(b0 + lane, s0) + BQ - 1) / BQ;
+      for (int b0 = 0; b0 < a.n; b0 += 64) {
+        const int m = rows_of(b0 + lane, s0);
+        if (__any(m < 0)) return t;
+        total += (m + BQ - 1) / BQ;
+      }
       for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
       total = uniform(total);
     } else {
@@ -116,6 +117,7 @@ __device__ Tile find_tile(const SinkArgs& a, int id) {
   for (int b0 = 0; b0 < a.n; b0 += 64) {
     int s0;
     const int m = rows_of(b0 + lane, s0), mine = (m + BQ - 1) / BQ * per;
+    if (__any(m < 0)) return t;
     int upto = mine;
     for (int o = 1; o < 64; o <<= 1) {
       const int u = __shfl_up(upto, o, 64);

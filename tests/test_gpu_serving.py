@@ -353,6 +353,13 @@ ATTEND = [
     ([9000], None, 4, 4, 64, 'fp8', 64, BF16, 5000, 8),
     ([700, 800, 900], None, 3, 3, 128, 'fp4', 64, BF16, 1, 300),
     ([1300], None, 64, 1, 64, 'fp4', 64, F16, None, 0),
+    # many sequences: shared out over the GPU, and a workgroup each; several tiles of rows on long tables
+    ([(37 * i) % 300 for i in range(90)] + [2500], None, 2, 2, 64, 'fp4', 64, BF16, None, 0),
+    ([(37 * i) % 300 for i in range(150)], None, 8, 8, 64, 'fp4', 32, BF16, 100, 3),
+    ([3000, 0, 40, 2500], [40, 0, 3, 21], 4, 2, 64, 'fp8', 16, BF16, None, 0),
+    ([3000, 2500], [30, 50], 8, 1, 128, 'fp4', 64, F16, 700, 90),
+    ([4000, 900, 0], None, 4, 2, 128, 'fp8', 64, F16, None, 0),
+    ([2300] * 3, [2, 1, 3], 1, 1, 128, 'fp8', 256, BF16, 2000, 4),
 ]
 P_CACHE = BF16  # bf16 queries' probabilities are rounded to bf16 in front of the values; fp16's are two bf16 terms
 
@@ -553,6 +560,34 @@ def test_steps_replay_from_graphs():
             for a, b in zip(out, step(window)):
                 assert torch.equal(a, b), (r, window)
         torch.cuda.synchronize()
+
+
+def test_sequences_that_share_one_table_row():
+    """A table expanded from one row, and lengths within it."""
+    f = Filled([400], 2, 64, 'fp4', 16, seed=43)
+    q = rows(torch.Generator().manual_seed(44), 3, 4, 64, BF16)
+    lens = [400, 17, 250]
+    got = f.cache.attend(q.to(DEV), f.table.expand(3, -1), i32(lens))
+    for b, n in enumerate(lens):
+        y, terms = plain.attend(q[b:b + 1], *f.held[0], torch.tensor([n - 1]), None, 0)
+        check(got[b:b + 1], y, terms, BF16, P_CACHE)
+    k, _ = f.cache.read(f.table.expand(3, -1), i32(lens), dtype=F32)
+    assert torch.equal(k.cpu(), torch.stack([f.held[0][0][n - 1] for n in lens]).float())
+
+
+def test_starts_that_decrease_compute_nothing_out_of_range():
+    """Starts are the caller's to keep; wrong ones leave rows unwritten, and nothing else is touched."""
+    f = Filled([300, 200], 2, 64, 'fp4', 64, seed=45)
+    q = rows(torch.Generator().manual_seed(46), 40, 4, 64, BF16).to(DEV)
+    bad = i32([0, 40, 0, 40, 7])
+    table, lens = f.table[[0, 1, 0, 1]].contiguous(), i32([300, 200, 300, 200])
+    out = torch.full_like(q, 5.0)
+    f.cache.attend(q, table, lens, bad, out=out)
+    ops.sink_attention(q, q[:, :2], q[:, :2], bad, out=out)
+    wide = torch.zeros(2, 5000, dtype=torch.int32, device=DEV)  # a long table: the rows are shared out
+    f.cache.attend(q, wide, i32([300, 200]), i32([0, 40, 3]), out=out)
+    f.cache.read(table, lens, bad, rows=40)
+    torch.cuda.synchronize()
 
 
 def test_another_stream():

@@ -28,7 +28,7 @@ def seqs(**kw):
 BAD_CACHES = [dict(keys=None), dict(values=None), dict(key_scales=None), dict(value_scales=None), dict(keys=8), dict(values=24),
               dict(key_scales=2), dict(pages=0), dict(pages=2 ** 31), dict(page_size=0), dict(page_size=8), dict(page_size=48),
               dict(page_size=512), dict(kv_heads=0), dict(kv_heads=2048), dict(dim=32), dict(dim=96), dict(format=2)]
-BAD_SEQS = [dict(table=None), dict(table_ld=1), dict(table_pages=-1), dict(lengths=None), dict(sequences=0), dict(rows=0),
+BAD_SEQS = [dict(table=None), dict(table_ld=-1), dict(table_pages=-1), dict(lengths=None), dict(sequences=0), dict(rows=0),
             dict(rows=4), dict(sequences=-1)]
 
 
