@@ -118,26 +118,19 @@ __device__ __forceinline__ int vswz(int R) {
   return DIM == 64 ? 2 * (((R >> 1) & 1) | ((((R >> 3) ^ R) & 1) << 1)) : 2 * ((R & 3) | (((R >> 3) & 1) << 2));
 }
 
-// max(a, b, c) in one instruction. (fmaxf first quiets each operand with an instruction of its own, as what left the matrix cores
-// could be a signalling NaN for all the compiler knows.)
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
-// The largest of a lane's scores, 4 N of them.
+// The largest of a lane's scores, 4 N of them: gfx950's three-operand maximum that passes a NaN on. (fmaxf first quiets each operand
+// with an instruction of its own, as what left the matrix cores could be a signalling NaN for all the compiler knows; and inline
+// assembly may not read it, since the compiler places the wait states that it needs in front of instructions it knows.)
 template <int N>
 __device__ __forceinline__ float max_scores(const f32x4 (&s)[N]) {
-  float m = max3(s[0][0], s[0][1], s[0][2]);
-  m = max3(m, s[0][3], s[0][3]);
+  float m = s[0][0];
 #pragma unroll
-  for (int x = 1; x < N; ++x) m = max3(max3(m, s[x][0], s[x][1]), s[x][2], s[x][3]);
+  for (int x = 1; x < 4 * N; ++x) m = __builtin_elementwise_maximum(m, s[x / 4][x % 4]);
   return m;
 }
 // The same over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float max_lanes4(float x) {
   const f32pair a = rowpair16(x);
-  const float y = max3(a.lo, a.hi, a.hi);
-  const f32pair b = halves32(y);
-  return max3(b.lo, b.hi, b.hi);
+  const f32pair b = halves32(__builtin_elementwise_maximum(a.lo, a.hi));
+  return __builtin_elementwise_maximum(b.lo, b.hi);
 }
