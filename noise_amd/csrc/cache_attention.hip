@@ -645,7 +645,8 @@ __global__ void __launch_bounds__(64 * NW) join_kernel(Args g) {
 }
 
 bool bad_attend(const Cache& c, const Sequences& s, const AttendArgs& a) {
-  return bad_cache(c, s) || (a.type != ROWS_BF16 && a.type != ROWS_F16) || a.heads <= 0 || a.heads > 1024 || a.heads % c.kv_heads || a.window < 0 || a.sinks < 0;
+  return bad_cache(c, s) || (a.type != ROWS_BF16 && a.type != ROWS_F16) || a.heads <= 0 || a.heads > 1024 ||
+         a.heads % c.kv_heads || a.window < 0 || a.sinks < 0;
 }
 
 // Whether pages hold whole blocks.
@@ -662,21 +663,24 @@ Shape shape_of(const Cache& c, const Sequences& s, const AttendArgs& a) {
   r.p.block_shift = c.dim == 64 ? 6 : 5;
   const long cap = (long)s.table_pages << c.page_shift;
   r.p.cap = (int)(cap < 0x7fffff00L ? cap : 0x7fffff00L);
-  // tiles: at most one begun by every sequence beside the full ones; no tile sees more blocks than the table names (and one more
-  // by alignment)
+  // tiles: at most one begun by every sequence beside the full ones; no tile sees more blocks than the table names, or its rows'
+  // windows and the sinks (and some more by alignment)
   const long full = (long)s.rows * r.p.group / RT;
   const long tiles = (s.starts ? full + (s.n < s.rows ? s.n : s.rows) : (long)s.rows * ((r.p.group + RT - 1) / RT)) * c.kv_heads;
-  const long blocks = (r.p.cap >> r.p.block_shift) + 2, fill = (long)resident(c.dim, c.format, a.type == ROWS_F16, wide_pages(c), s.starts) * num_cus();
-  // A workgroup a tile, and no second kernel, where a table names so few keys that this costs no more than sharing them out (a
+  const long all = r.p.cap >> r.p.block_shift, some = (((long)a.window + RT + 1) >> r.p.block_shift) + 1 + (a.sinks >> r.p.block_shift) + 1;
+  const long blocks = (some < all ? some : all) + 2;
+  const long fill = (long)resident(c.dim, c.format, a.type == ROWS_F16, wide_pages(c), s.starts) * num_cus();
+  // A workgroup a tile, and no second kernel, where a tile sees so few keys that this costs no more than sharing them out (a
   // round takes about 1.4 us): 11 blocks of 8 heads on eight waves 8.2 us, shared 7.3 + 4.4; 64 sequences of 33 blocks 20.8,
-  // shared 23.8 + 4.8; but one of 63 blocks 17.5, shared 7.3 + 5.7. Also where there are many tiles, or more rounds than fit.
+  // shared 23.8 + 4.8; 8 drafts of each of 32 sequences in windows of 2048 keys 15.1, shared 15.8 + 5.8; but one sequence of 63
+  // blocks 17.5, shared 7.3 + 5.7. Also where there are many tiles, or more rounds than fit.
   r.items = tiles;
   r.p.waves = 4;
-  if (blocks <= 34 && tiles <= num_cus()) {
+  if (blocks <= 40 && tiles <= 2 * num_cus()) {
     r.p.waves = 8;
     return r;
   }
-  if (blocks <= 18 || (blocks <= 66 && tiles >= fill / 2) || tiles >= 32 * fill || tiles * blocks > 0x3fffffffL) return r;
+  if (blocks <= 18 || (blocks <= 66 && tiles >= fill / 2) || tiles >= 32 * fill || tiles * (all + 2) > 0x3fffffffL) return r;
   const long most = tiles * ((blocks + r.p.waves - 1) / r.p.waves);
   r.items = r.p.groups = (int)(most < fill ? most : fill);
   return r;
@@ -687,8 +691,11 @@ size_t part_bytes(const Cache& c, const Shape& r) { return (size_t)r.p.groups * 
 }  // namespace
 
 int cache_attend_workspace(const Cache& c, const Sequences& s, const AttendArgs& a, size_t* bytes) {
-  if (bad_attend(c, s, a)) return NOISE_EINVAL;
-  const Shape r = shape_of(c, s, a);
+  // (for any window and sinks: a short window may need none)
+  AttendArgs all = a;
+  all.window = 0x7fffffff;
+  if (bad_attend(c, s, all)) return NOISE_EINVAL;
+  const Shape r = shape_of(c, s, all);
   *bytes = part_bytes(c, r) + (size_t)r.p.groups * 2 * RT * 8;
   return NOISE_OK;
 }
@@ -698,8 +705,7 @@ int cache_attend_launch(const Cache& c, const Sequences& s, const AttendArgs& a,
   if (bad_attend(c, s, a) || bad_heads(a.q) || !a.y || ((uintptr_t)a.y & 15) || !(a.scale >= 0.f) || a.scale > 3.4e38f)
     return NOISE_EINVAL;
   const Shape r = shape_of(c, s, a);
-  size_t need = 0;
-  cache_attend_workspace(c, s, a, &need);
+  const size_t need = part_bytes(c, r) + (size_t)r.p.groups * 2 * RT * 8;
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) return NOISE_ENOSPC;
   Args g{c, s, a, r.p, 0.f, 0, 0, nullptr, nullptr};
   // (a scale of 0 is the smallest normal number: every seen key weighs the same, and a masked score stays -infinity)

@@ -360,6 +360,9 @@ ATTEND = [
     ([3000, 2500], [30, 50], 8, 1, 128, 'fp4', 64, F16, 700, 90),
     ([4000, 900, 0], None, 4, 2, 128, 'fp8', 64, F16, None, 0),
     ([2300] * 3, [2, 1, 3], 1, 1, 128, 'fp8', 256, BF16, 2000, 4),
+    # windows of more blocks than a workgroup takes alone, and of fewer on long tables
+    ([4100, 3900, 10], [20, 1, 3], 4, 2, 64, 'fp4', 32, BF16, 2700, 70),
+    ([4100, 3900, 10], [20, 1, 3], 16, 2, 64, 'fp8', 64, F16, 200, 70),
 ]
 P_CACHE = BF16  # bf16 queries' probabilities are rounded to bf16 in front of the values; fp16's are two bf16 terms
 
