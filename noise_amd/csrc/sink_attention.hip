@@ -2,10 +2,13 @@
 // j < sinks. Sequences of any lengths are packed in one call, heads may be grouped over fewer kv heads.
 //
 // Bound: for dim 64 the softmax's vector work (an exponential, a fused multiply-add, half a maximum and half a conversion a score,
-// beside 4 x 64 flop on the matrix cores), for dim 128 the matrix cores.
+// beside 4 x 64 flop on the matrix cores), for dim 128 the matrix cores: 16384 tokens of 8 heads take 338 us (813 TFLOP/s of the
+// seen scores) and 568 us (968 TFLOP/s; a matrix product of 8192^3 reaches 1248). Short windows pay for blocks seen in part and
+// for beginnings: 16 sequences of 2048 tokens in windows of 1024 88 us (590 TFLOP/s).
 //
 // One workgroup takes 64 QB queries of one sequence and head, a wave 16 QB of them; key blocks of 64 go through a double-buffered
-// LDS ring by direct global -> LDS loads, block j + 1 landing while block j is computed.
+// LDS ring by direct global -> LDS loads, block j + 1 landing while block j is computed (a third slot, two blocks on their way,
+// changed no time by more than 5% either way). With few tiles a second group of four waves takes every other block.
 //   S^T = K Q^T (A = K rows, B = Q rows): a lane holds 16 scores of query lane % 16. K rows are interleaved at load time so that
 //   the scores' layout is the B operand of O^T += V^T P^T: P never leaves registers. V stays row-major [key][channel] and
 //   its A fragments come from transposing LDS reads.
@@ -121,8 +124,9 @@ __device__ Tile find_tile(const SinkArgs& a, int id) {
   return t;
 }
 
-template <int DIM, bool F16, int QB>
-__global__ void __launch_bounds__(NTH, DIM == 64 ? 3 : 2) sink_kernel(Args g) {
+// KS groups of four waves, each with a KS-th of the tile's key blocks.
+template <int DIM, bool F16, int QB, int KS>
+__global__ void __launch_bounds__(NTH * KS, DIM == 128 ? 2 : KS == 2 ? 4 : 3) sink_kernel(Args g) {
   using E = Elem<F16>;
   using T = typename E::T;
   using x8 = typename E::x8;
@@ -131,14 +135,15 @@ __global__ void __launch_bounds__(NTH, DIM == 64 ? 3 : 2) sink_kernel(Args g) {
   constexpr int ROWB = 2 * DIM, CH = DIM / 8;          // bytes and 16-byte chunks of a row
   constexpr int DH = BKV * ROWB / 1024 / NWAVE;        // load instructions of 1 KiB per wave, block and operand
   constexpr int RPI = 1024 / ROWB;                     // rows of one
-  __shared__ __attribute__((aligned(1024))) char sk[2][BKV * ROWB];
-  __shared__ __attribute__((aligned(1024))) char sv[2][BKV * ROWB];
+  __shared__ __attribute__((aligned(1024))) char sk[KS][2][BKV * ROWB];
+  __shared__ __attribute__((aligned(1024))) char sv[KS][2][BKV * ROWB];
   const SinkArgs& a = g.a;
   if ((int)blockIdx.x >= g.items) {
-    fill_rows(a.starts, a.n, a.rows, a.y, a.heads * DIM, NTH, blockIdx.x - g.items, g.fills);
+    fill_rows(a.starts, a.n, a.rows, a.y, a.heads * DIM, NTH * KS, blockIdx.x - g.items, g.fills);
     return;
   }
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = lane >> 4, r16 = lane & 15;
+  const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4, r16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NWAVE, part = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 8);
   const Tile w = find_tile<BQ>(a, blockIdx.x);
   if (!w.found) return;
   const int kh = w.h / (a.heads / a.kv_heads), last = w.m - 1;
@@ -172,7 +177,7 @@ __global__ void __launch_bounds__(NTH, DIM == 64 ? 3 : 2) sink_kernel(Args g) {
     // (opaque here and in block(): what is derived from these would be kept in registers over the loop)
     asm volatile("" : "+v"(kr0), "+v"(vr0), "+v"(kc0), "+v"(vc0));
     const char *k0 = kp + (long)j0 * kld, *v0 = vp + (long)j0 * vld;
-    const char *kd = sk[buf] + DH * wave * 1024, *vd = sv[buf] + DH * wave * 1024;
+    const char *kd = sk[part][buf] + DH * wave * 1024, *vd = sv[part][buf] + DH * wave * 1024;
 #pragma unroll
     for (int q = 0; q < DH; ++q)
       dma_x4_s(k0, __umul24(min(kr0 + (DIM == 64 ? 16 : 8) * q, lim), kld) + (DIM == 64 ? kc0 : kc0 ^ (64 * q)), kd + 1024 * q);
@@ -194,11 +199,11 @@ __global__ void __launch_bounds__(NTH, DIM == 64 ? 3 : 2) sink_kernel(Args g) {
     constexpr int buf = decltype(bufc)::value;
     constexpr bool CAREFUL = decltype(carefulc)::value;
     const int j0 = block_key(i);
-    const char *kt = sk[buf], *vt = sv[buf];
+    const char *kt = sk[part][buf], *vt = sv[part][buf];
     asm volatile("" : "+v"(kro), "+v"(vro));
     // blocks that this wave's queries see not at all, or in part
     if (j0 > qe || (qw - (j0 + BKV - 1) > a.window && j0 >= a.sinks)) return;
-    const bool part = j0 + BKV - 1 > qw || (qe - j0 > a.window && j0 + BKV > a.sinks);
+    const bool some = j0 + BKV - 1 > qw || (qe - j0 > a.window && j0 + BKV > a.sinks);
     f32x4 s[QB][KB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -212,7 +217,7 @@ __global__ void __launch_bounds__(NTH, DIM == 64 ? 3 : 2) sink_kernel(Args g) {
         for (int q = 0; q < QS; ++q) s[qb][kb] = mfma<F16>(kf[q], qf[qb][q], s[qb][kb]);
       }
     }
-    if (part) {
+    if (some) {
       // key j0 + 8 grp + t, t a constant, of query j0 + 8 grp + top: seen when 0 <= top - t <= window or t <= top, t < sinks'
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
@@ -304,11 +309,12 @@ __global__ void __launch_bounds__(NTH, DIM == 64 ? 3 : 2) sink_kernel(Args g) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) osum[qb] = mfma<F16>(ones, pf[qb][c], osum[qb]);
   };
-  // Block i + 1 lands in the other slot while block i is computed; then it has landed for this wave, and the barrier makes every
-  // wave's part of it visible and retires block i's slot. (The loads are the only vector memory operations in flight.)
+  // Each group of waves takes every KS-th block: its next one lands in its other slot while one is computed; then it has landed for
+  // this wave, and the barrier makes every wave's part of it visible and retires the slot. (The loads are the only vector memory
+  // operations in flight.)
   auto step = [&](int i, auto bufc, auto carefulc) {
-    if (i + 1 < blocks) issue(i + 1, decltype(bufc)::value ^ 1);
-    block(i, bufc, carefulc);
+    if (i + part + KS < blocks) issue(i + part + KS, decltype(bufc)::value ^ 1);
+    if (KS == 1 || i + part < blocks) block(i + part, bufc, carefulc);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   };
@@ -320,12 +326,12 @@ __global__ void __launch_bounds__(NTH, DIM == 64 ? 3 : 2) sink_kernel(Args g) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[qb][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    issue(0, 0);
+    if (part < blocks) issue(part, 0);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    for (int i = 0; i < blocks; i += 2) {
+    for (int i = 0; i < blocks; i += 2 * KS) {
       step(i, std::integral_constant<int, 0>{}, carefulc);
-      if (i + 1 < blocks) step(i + 1, std::integral_constant<int, 1>{}, carefulc);
+      if (i + KS < blocks) step(i + KS, std::integral_constant<int, 1>{}, carefulc);
     }
   };
   pass(std::false_type{});
@@ -339,6 +345,27 @@ __global__ void __launch_bounds__(NTH, DIM == 64 ? 3 : 2) sink_kernel(Args g) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) odd |= !(fabsf(o[qb][d][e]) < INFINITY);
   if (__syncthreads_or(odd)) pass(std::true_type{});
+
+  if constexpr (KS == 2) {
+    // the second group's sums join the first's through LDS (its K slots: 16 DIM floats a wave)
+    static_assert(QB == 1);
+    f32x4* to = reinterpret_cast<f32x4*>(sk[1][0]) + wave * DT * 64 + lane;
+    float2* ml = reinterpret_cast<float2*>(sv[1][0]) + wave * 64 + lane;
+    if (part) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) to[64 * d] = o[0][d];
+      *ml = make_float2(mref[0], osum[0][0]);
+    }
+    __syncthreads();
+    if (part) return;
+    // (a row may see none of one group's blocks, which then has no maximum and sums of zero; its own key is in the other's)
+    const float m1 = ml->x, l1 = ml->y, m = fmaxf(mref[0], m1);
+    const float a0 = mref[0] == m ? 1.f : __builtin_amdgcn_exp2f((mref[0] - m) * g.c2);
+    const float a1 = m1 == m ? 1.f : __builtin_amdgcn_exp2f((m1 - m) * g.c2);
+    osum[0][0] = osum[0][0] * a0 + l1 * a1;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[0][d] = o[0][d] * a0 + to[64 * d] * a1;
+  }
 
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
@@ -368,19 +395,26 @@ int sink_attention_launch(const SinkArgs& a, hipStream_t stream) {
     const long tiles = a.starts ? a.rows / bq + (a.n < a.rows ? a.n : a.rows) : (long)a.n * ((a.T + bq - 1) / bq);
     return a.heads % 8 == 0 ? tiles * a.heads : (tiles * a.heads + 7) / 8 * 8;
   };
-  const bool narrow = groups(128) <= 2 * num_cus();
+  // Tiles of 64 queries where those of 128 leave the GPU empty for much of the time, and two groups of waves where those do too (8
+  // heads, one sequence unless said otherwise; 128 queries / 64 / 64 in two groups. dim 64: 1000 tokens 20 / 14.3 / 12.0 us, 2048 34 /
+  // 24.4 / 20.0, 6000 95 / 74 / 67, 8192 132 / 107 / 109, 4 of 2048 in windows of 1024 30.5 / 27.8 / 32.9, 2 of 6000 43.5 / 44.3 / 52;
+  // dim 128: 2048 46 / 36 / 28, 4096 88 / 73 / 61, 6000 135 / 110 / 129, 8192 187 / 192, 4 of 2048 in windows 45.5 / 54).
+  const long tiles = groups(128), cus = num_cus();
+  const bool narrow = tiles <= (a.dim == 64 ? 3 : 2) * cus, split = 4 * tiles <= (a.dim == 64 ? 6 : 5) * cus;
   const long items = groups(narrow ? 64 : 128);
   Args g{a, 0.f, (int)items, a.fill && a.starts ? 32 : 0};
   if (items + g.fills > 0x7fffffffL) return NOISE_ENOTSUP;
   // (a scale of 0 is the smallest normal number: every seen key weighs the same, and a masked score stays -infinity)
   const float c2 = a.scale * 1.4426950408889634f;
   g.c2 = c2 > 1.17549435e-38f ? c2 : 1.17549435e-38f;
-  auto launch = [&](auto dim, auto f16_, auto qb) {
-    hipLaunchKernelGGL((sink_kernel<decltype(dim)::value, decltype(f16_)::value, decltype(qb)::value>),
-                       dim3((unsigned)(items + g.fills)), dim3(NTH), 0, stream, g);
+  auto launch = [&](auto dim, auto f16_, auto qb, auto ks) {
+    hipLaunchKernelGGL((sink_kernel<decltype(dim)::value, decltype(f16_)::value, decltype(qb)::value, decltype(ks)::value>),
+                       dim3((unsigned)(items + g.fills)), dim3(NTH * decltype(ks)::value), 0, stream, g);
   };
+  const std::integral_constant<int, 1> one{};
+  const std::integral_constant<int, 2> two{};
   auto with = [&](auto dim, auto f16_) {
-    narrow ? launch(dim, f16_, std::integral_constant<int, 1>{}) : launch(dim, f16_, std::integral_constant<int, 2>{});
+    split ? launch(dim, f16_, one, two) : narrow ? launch(dim, f16_, one, one) : launch(dim, f16_, two, one);
   };
   const std::integral_constant<int, 64> d64{};
   const std::integral_constant<int, 128> d128{};

@@ -83,6 +83,42 @@ def test_prompts_match_the_plain_form(case):
     check(got, y, terms, dtype, dtype)
 
 
+# (tiles of 64 queries by one group of waves, and of 128 queries: many heads)
+@pytest.mark.parametrize('case', [
+    ([700, 0, 301, 1], 64, 8, 64, BF16, 200, 5),
+    ([900, 60], 64, 64, 64, F16, None, 0),
+    ([700, 0, 501], 32, 4, 128, BF16, 200, 5),
+    ([129, 0, 301, 1] + [70] * 12, 64, 8, 64, F16, 100, 5),
+    ([1000, 257], 80, 16, 64, BF16, None, 0),
+    ([513, 300, 64], 100, 4, 128, BF16, None, 0),
+    ([30, 1, 200] + [65] * 70, 6, 2, 128, F16, 50, 2),
+], ids=str)
+def test_prompts_of_many_tiles(case):
+    log_case(f'prompt {case}')
+    lens, *_, dtype, window, sinks = case
+    q, k, v = prompt(case, 5)
+    y, terms = prompt_reference(q, k, v, lens, window, sinks)
+    got = ops.sink_attention(q.to(DEV), k.to(DEV), v.to(DEV), i32(starts_of(lens)), window=window, sinks=sinks)
+    check(got, y, terms, dtype, dtype)
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+@pytest.mark.parametrize('heads', [4, 64, 128])
+def test_unseen_values_in_every_kind_of_tile(heads, bad):
+    """Values that come after a row, and before its window, hold NaN or infinities: rows that see none of them are what they were."""
+    lens, window, n = [300, 400], 60, 700
+    q, k, v = prompt((lens, heads, 1, 64, BF16, window, 0), 8)
+    want = ops.sink_attention(q.to(DEV), k.to(DEV), v.to(DEV), i32(starts_of(lens)), window=window).cpu()
+    v[250:300] = bad
+    v[500] = bad
+    got = ops.sink_attention(q.to(DEV), k.to(DEV), v.to(DEV), i32(starts_of(lens)), window=window).cpu()
+    clean = torch.ones(n, dtype=torch.bool)
+    clean[250:300] = False
+    clean[500:500 + window + 1] = False
+    assert (got[clean] - want[clean]).abs().max() <= 2 ** -7 * want.abs().max()  # (sums in another order: a rounding either way)
+    assert not torch.isfinite(got[~clean]).any()
+
+
 def test_prompt_batches_are_packed_sequences():
     """[batch, T, heads, dim] gives the bits of the packed call; fused and padded strides are read in place."""
     g = torch.Generator().manual_seed(3)
