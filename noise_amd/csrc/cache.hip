@@ -11,7 +11,8 @@
 // turns them over in LDS: the rows are read or written in their own order (a lane 8 channels, 16 or 32 bytes; the four
 // lanes of a group share its maximum through DPP), the codes in the cache's, head by head, where consecutive tokens of a page
 // are consecutive bytes (a lane 16 bytes). Reading 64 bytes of a head here and there between the stores instead, without LDS, took
-// 24 sequences of up to 8192 tokens, 8 heads of 128 in e2m1, 137 us where their stores alone take 85.
+// 24 sequences of up to 8192 tokens, 8 heads of 128 in e2m1, 137 us where their stores alone take 85. Now 111 us, 5.1 TB/s, as a large
+// copy; 32 prompts of up to 2048 rows, 8 heads of 64 in fp16 to e4m3, are written in 23 us and read in 23 (4.0 TB/s).
 #include <type_traits>
 
 #include "common.h"

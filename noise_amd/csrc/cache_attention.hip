@@ -3,7 +3,9 @@
 //
 // Bound: the visible tokens' bytes, read once per kv head (dim 64: 68 bytes a token in e2m1). The rows of one sequence and kv
 // head, at most 16 (new tokens x query heads of the group), are the columns of one MFMA tile, so a group of heads costs what
-// one head costs, and idle columns are free while memory is the bound.
+// one head costs, and idle columns are free while memory is the bound. 48 sequences of up to 32768 tokens, 8 heads of 64 in e2m1, take
+// 92 us (4.95 TB/s of what they see), 200000 tokens in e4m3 44 us (4.8 TB/s), a join 5 to 7 us more; 16 sequences of up to 16384,
+// 32 heads over 4 of 128 in e2m1, 23 us (3.4 TB/s: start-up). A step of one short sequence takes 7 us, a few round trips to memory.
 //
 // A wave takes blocks of BK keys (64 of dim 64, 32 of dim 128) with its own running maximum and sum:
 //   K codes go from global memory to registers (a lane holds a quarter of a key's channels, all of one scale group) and become
