@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import ROW_TYPES, _ptr, heads_rows, launch, mask_args, no_grad_rows, one_device, output_rows, sequence_starts
+from .ops import ROW_TYPES, _ptr, heads_rows, launch, mask_args, no_grad_rows, one_device, output_rows, row_count, sequence_starts
 
 FORMATS = {'fp4': _lib.CACHE_FP4, 'fp8': _lib.CACHE_FP8}
 
@@ -65,6 +65,7 @@ class KVCache:
 
     def _sequences(self, table, lengths, starts, rows):
         """noise_sequences_t of a call's tensors (kept alive by the caller until the call is enqueued)."""
+        row_count(rows)
         one_device(self.keys, table, lengths)
         if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError('table must be an int32 tensor [sequences, pages of a sequence] with contiguous rows')
@@ -104,8 +105,6 @@ class KVCache:
             if starts is not None:
                 raise ValueError('rows must be given with starts')
             rows = table.shape[0]
-        if rows < 0 or rows >= 2 ** 31:
-            raise ValueError(f'rows must lie in [0, 2^31), got {rows}')
         seqs = self._sequences(table, lengths, starts, rows)
         shape = (rows, self.kv_heads, self.dim)
         if not seqs.sequences:

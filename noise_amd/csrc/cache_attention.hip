@@ -664,7 +664,7 @@ Shape shape_of(const Cache& c, const Sequences& s, const AttendArgs& a) {
   r.p.group = a.heads / c.kv_heads;
   r.p.block_shift = c.dim == 64 ? 6 : 5;
   const long cap = (long)s.table_pages << c.page_shift;
-  r.p.cap = (int)(cap < 0x7fffff00L ? cap : 0x7fffff00L);
+  r.p.cap = (int)(cap < POSITIONS ? cap : POSITIONS);
   // tiles: at most one begun by every sequence beside the full ones; no tile sees more blocks than the table names, or its rows'
   // windows and the sinks (and some more by alignment)
   const long full = (long)s.rows * r.p.group / RT;

@@ -84,10 +84,12 @@ __device__ __forceinline__ int find_sequence(const int* starts, int n, int i) {
   return lo + __builtin_popcountll(m);
 }
 
+constexpr int POSITIONS = 0x7fffff00;  // a position's limit: sums with a block's keys stay within an int
+
 // The slot (page * page size + token) of a position, or -1 where the table names no page of the cache for it.
 __device__ __forceinline__ long slot_of(const Cache& c, const Sequences& s, int b, long pos) {
   const long pg = pos >> c.page_shift;
-  if (pos < 0 || pg >= s.table_pages) return -1;
+  if (pos < 0 || pos >= POSITIONS || pg >= s.table_pages) return -1;
   const int id = s.table[b * s.table_ld + pg];
   if (id < 0 || id >= c.pages) return -1;
   return ((long)id << c.page_shift) + (pos & ((1 << c.page_shift) - 1));

@@ -150,15 +150,23 @@ def one_device(*tensors):
     return dev
 
 
-def heads_rows(t):
+def row_count(rows):
+    """Checks a call's number of packed rows, an int of the entry points."""
+    if not 0 <= rows < 2 ** 31:
+        raise ValueError(f'rows must lie in [0, 2^31), got {rows}')
+    return rows
+
+
+def heads_rows(t, below=2 ** 63):
     """(tensor to keep alive, pointer, row stride, head stride) of rows [n, heads, dim] as the kernels read them: in place
-    where the channels are contiguous and rows and heads start at 16-byte addresses, else from a contiguous copy."""
+    where the channels are contiguous, rows and heads start at 16-byte addresses and the row stride is less than `below`, else
+    from a contiguous copy."""
     unit = 16 // t.element_size()
     n, heads, dim = t.shape
     ld, hs, one = t.stride()
     # (the stride of a dimension of one entry means nothing)
     ld, hs, p = ld if n > 1 else 0, hs if heads > 1 else 0, t.data_ptr()
-    if one != 1 or ld % unit or hs % unit or p % 16:
+    if one != 1 or ld % unit or hs % unit or p % 16 or ld >= below:
         t = t.clone(memory_format=torch.contiguous_format)
         ld, hs, p = heads * dim, dim, t.data_ptr()
     return t, p, ld, hs
@@ -218,6 +226,7 @@ def sink_attention(q, k, v, starts=None, window=None, sinks=0, scale=None, out=N
     if dim not in (64, 128) or kv == 0 or heads == 0 or heads % kv or heads > 1024:
         raise ValueError(f'dim must be 64 or 128 and heads (at most 1024) a multiple of kv_heads: got {heads} x {dim} on {kv}')
     window, sinks, scale = mask_args(window, sinks, scale, dim)
+    rows = row_count(math.prod(q.shape[:-2]))
     y, fill = output_rows(out, q, dev)
     T = 0
     if starts is None:
@@ -225,14 +234,13 @@ def sink_attention(q, k, v, starts=None, window=None, sinks=0, scale=None, out=N
         q, k, v = q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1)
     else:
         n = sequence_starts(starts, dev)
-    rows = q.shape[0]
     if rows == 0:
         return y
     if n == 0:  # no sequence at all: every row is behind the last one
         return y.zero_() if fill else y
     q, qp, ql, qh = heads_rows(q)
-    k, kp, kl, kh = heads_rows(k)
-    v, vp, vl, vh = heads_rows(v)
+    k, kp, kl, kh = heads_rows(k, 2 ** 23)
+    v, vp, vl, vh = heads_rows(v, 2 ** 23)
     launch(dev, 'noise_sink_attention', qp, ql, qh, kp, kl, kh, vp, vl, vh, _ptr(starts), n, rows, T, heads, kv, dim,
            ROW_TYPES[q.dtype], window, sinks, scale, y.data_ptr(), fill)
     return y

@@ -132,6 +132,10 @@ def test_prompt_batches_are_packed_sequences():
     assert torch.equal(ops.sink_attention(f[:, 0], f[:, 1], f[:, 2], i32([0, T, 2 * T, 3 * T]), window=70, sinks=2), want)
     odd = [torch.cat((torch.zeros(B * T, H, 3, device=DEV, dtype=BF16), x), -1)[:, :, 3:] for x in packed]  # not 16-byte rows
     assert torch.equal(ops.sink_attention(*odd, i32([0, T, 2 * T, 3 * T]), window=70, sinks=2), want)
+    far = torch.zeros(2, 2 ** 23 + 64, device=DEV, dtype=BF16).as_strided((2, 1, 64), (2 ** 23, 64, 1))  # rows far apart
+    far.copy_(packed[1][:2, :1])
+    pair = ops.sink_attention(packed[0][:2], packed[1][:2, :1], packed[2][:2, :1], i32([0, 2]))
+    assert torch.equal(ops.sink_attention(packed[0][:2], far, packed[2][:2, :1], i32([0, 2])), pair)
     shared = packed[1][:, :1].expand(-1, H, -1)  # one kv head broadcast to all
     one = ops.sink_attention(packed[0], packed[1][:, :1], packed[2][:, :1], i32([0, B * T]))
     assert torch.equal(ops.sink_attention(packed[0], shared, packed[2][:, :1].expand(-1, H, -1), i32([0, B * T])), one)
@@ -502,6 +506,32 @@ def test_far_pages():
     got = cache.read(table, i32([n]), i32([0, n]), rows=n, dtype=F32)
     assert torch.equal(got[0].cpu(), hk.float()) and torch.equal(got[1].cpu(), hv.float())
     assert not cache.keys[:40].any()
+
+
+def test_last_positions():
+    """Positions from 2^31 - 256 on are bad places to all three, whatever the table names for them; the ones in front are not."""
+    cache = KVCache.zeros(4, kv_heads=1, dim=64, page_size=256, format='fp8')
+    table = torch.zeros(1, 2 ** 23, device=DEV, dtype=torch.int32)  # every position's page is page 0, but the last three
+    last = 2 ** 31 - 256
+    table[0, -2], table[0, -1] = 1, 2
+    x = torch.full((3, 1, 64), 2., device=DEV, dtype=BF16)
+    cache.write(x, x, table, i32([last + 2]), i32([0, 3]))  # the last position in front, and two behind
+    assert cache.values[1, 0, 255].all() and not cache.values[2].any()
+    k, v = cache.read(table, i32([last + 2]), i32([0, 3]), rows=3)
+    assert torch.equal(v[0], x[0]) and torch.isnan(v[1:]).all() and torch.isnan(k[1:]).all()
+    y = cache.attend(x, table, i32([last + 2]), i32([0, 3]), window=0)
+    assert torch.equal(y[0], x[0]) and torch.isnan(y[1:]).all()
+
+
+def test_more_rows_than_a_call_takes_are_refused():
+    cache = KVCache.zeros(1, kv_heads=1, page_size=16)
+    x = torch.zeros(1, 1, 64, device=DEV, dtype=BF16).expand(2 ** 31, 1, 64)
+    table, lengths, st = torch.zeros(1, 1, device=DEV, dtype=torch.int32), i32([5]), i32([0, 2])
+    for call in (lambda: ops.sink_attention(x, x, x, st), lambda: ops.sink_attention(*[x.unsqueeze(0)] * 3),
+                 lambda: cache.write(x, x, table, lengths, st), lambda: cache.attend(x, table, lengths, st),
+                 lambda: cache.read(table, lengths, st, rows=2 ** 31), lambda: cache.read(table, lengths, st, rows=-1)):
+        with pytest.raises(ValueError, match='rows must lie'):
+            call()
 
 
 def test_cache_types_and_shapes_are_refused():
