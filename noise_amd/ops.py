@@ -122,7 +122,7 @@ NO_WINDOW = 2 ** 31 - 1
 
 def launch(dev, name, *args):
     """Calls an entry point on device dev, on its current stream (the last argument)."""
-    if torch.cuda.current_device() == dev.index:
+    if torch._C._cuda_getDevice() == dev.index:
         _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
@@ -131,12 +131,9 @@ def launch(dev, name, *args):
 
 def no_grad_rows(*tensors):
     """The serving operators are forward-only: refuse a tensor whose gradient a caller would expect."""
-    if not torch.is_grad_enabled():
-        return
     for t in tensors:
-        if not t.requires_grad:
-            continue
-        raise RuntimeError('the serving operators have no backward pass: call them under torch.no_grad() or detach the inputs')
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError('the serving operators have no backward pass: call them under torch.no_grad() or detach the inputs')
 
 
 def one_device(*tensors):
@@ -161,11 +158,14 @@ def heads_rows(t, below=2 ** 63):
     """(tensor to keep alive, pointer, row stride, head stride) of rows [n, heads, dim] as the kernels read them: in place
     where the channels are contiguous, rows and heads start at 16-byte addresses and the row stride is less than `below`, else
     from a contiguous copy."""
-    unit = 16 // t.element_size()
+    unit = 16 // t.itemsize
     n, heads, dim = t.shape
     ld, hs, one = t.stride()
-    # (the stride of a dimension of one entry means nothing)
-    ld, hs, p = ld if n > 1 else 0, hs if heads > 1 else 0, t.data_ptr()
+    p = t.data_ptr()
+    if n == 1:  # (the stride of a dimension of one entry means nothing)
+        ld = 0
+    if heads == 1:
+        hs = 0
     if one != 1 or ld % unit or hs % unit or p % 16 or ld >= below:
         t = t.clone(memory_format=torch.contiguous_format)
         ld, hs, p = heads * dim, dim, t.data_ptr()
@@ -217,20 +217,20 @@ def sink_attention(q, k, v, starts=None, window=None, sinks=0, scale=None, out=N
     dev = one_device(q, k, v)
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f'q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}')
-    nd = 4 if starts is None else 3
-    if q.dim() != nd or k.shape != v.shape or k.dim() != nd or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+    qs, ks = q.shape, k.shape
+    if len(qs) != (4 if starts is None else 3) or ks != v.shape or ks[:-2] != qs[:-2] or ks[-1] != qs[-1]:
         raise ValueError('q must be [n, heads, dim] and k, v [n, kv_heads, dim] with starts, [batch, T, ...] without; got '
-                         f'{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
-    heads, dim = q.shape[-2:]
-    kv = k.shape[-2]
+                         f'{tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}')
+    *_, heads, dim = qs
+    kv = ks[-2]
     if dim not in (64, 128) or kv == 0 or heads == 0 or heads % kv or heads > 1024:
         raise ValueError(f'dim must be 64 or 128 and heads (at most 1024) a multiple of kv_heads: got {heads} x {dim} on {kv}')
     window, sinks, scale = mask_args(window, sinks, scale, dim)
-    rows = row_count(math.prod(q.shape[:-2]))
+    rows = row_count(qs[0] if starts is not None else qs[0] * qs[1])
     y, fill = output_rows(out, q, dev)
     T = 0
     if starts is None:
-        n, T = q.shape[:2]
+        n, T = qs[:2]
         q, k, v = q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1)
     else:
         n = sequence_starts(starts, dev)
