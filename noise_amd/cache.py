@@ -63,14 +63,21 @@ class KVCache:
         t = [torch.zeros(pages, kv_heads, page_size, n, dtype=torch.uint8, device=device) for n in (width, dim // 32) * 2]
         return cls(*t)
 
+    def _beside(self, *tensors):
+        """Checks that all are on the cache's device."""
+        for t in tensors:
+            if t.device != self.device:
+                one_device(self.keys, t)
+
     def _sequences(self, table, lengths, starts, rows):
         """noise_sequences_t of a call's tensors (kept alive by the caller until the call is enqueued)."""
         row_count(rows)
-        one_device(self.keys, table, lengths)
-        if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        self._beside(table, lengths)
+        dims = table.shape
+        if table.dtype != torch.int32 or len(dims) != 2 or (dims[1] > 1 and table.stride(1) != 1):
             raise ValueError('table must be an int32 tensor [sequences, pages of a sequence] with contiguous rows')
-        n, pages = table.shape
-        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (n,) or not lengths.is_contiguous():
+        n, pages = dims
+        if lengths.dtype != torch.int32 or lengths.shape != (n,) or not lengths.is_contiguous():
             raise ValueError(f'lengths must be a contiguous int32 vector of {n} entries')
         if starts is None:
             if rows != n:
@@ -83,10 +90,10 @@ class KVCache:
         """Quantises the rows k and v [n, kv_heads, dim] (bf16, fp16 or fp32, any strides) into their places. The places of one
         call must be distinct: two sequences may share pages that neither writes."""
         no_grad_rows(k, v)
-        one_device(self.keys, k, v)
+        self._beside(k, v)
         if k.dtype not in ROW_TYPES or v.dtype != k.dtype:
             raise TypeError(f'k and v must be bfloat16, float16 or float32 alike, got {k.dtype} and {v.dtype}')
-        if k.dim() != 3 or tuple(k.shape[1:]) != (self.kv_heads, self.dim) or v.shape != k.shape:
+        if len(k.shape) != 3 or k.shape[1:] != (self.kv_heads, self.dim) or v.shape != k.shape:
             raise ValueError(f'k and v must be [n, {self.kv_heads}, {self.dim}], got {tuple(k.shape)} and {tuple(v.shape)}')
         seqs = self._sequences(table, lengths, starts, k.shape[0])
         if not seqs.rows or not seqs.sequences:
@@ -121,23 +128,24 @@ class KVCache:
         values of their sequences: a query at position s sees the keys j <= s with s - j <= window (None: all) or j < sinks.
         Masks, scale, zero rows and `out` as in noise_amd.ops.sink_attention; a row that sees a bad place is NaN."""
         no_grad_rows(q)
-        one_device(self.keys, q)
+        self._beside(q)
         if q.dtype not in (torch.bfloat16, torch.float16):
             raise TypeError(f'q must be bfloat16 or float16, got {q.dtype}')
-        if q.dim() != 3 or q.shape[2] != self.dim or q.shape[1] == 0 or q.shape[1] % self.kv_heads or q.shape[1] > 1024:
+        dims = q.shape
+        if len(dims) != 3 or dims[2] != self.dim or dims[1] == 0 or dims[1] % self.kv_heads or dims[1] > 1024:
             raise ValueError(f'q must be [n, heads, {self.dim}] with heads (at most 1024) a multiple of {self.kv_heads}, got '
-                             f'{tuple(q.shape)}')
+                             f'{tuple(dims)}')
         window, sinks, scale = mask_args(window, sinks, scale, self.dim)
-        seqs = self._sequences(table, lengths, starts, q.shape[0])
+        rows, heads, _ = dims
+        seqs = self._sequences(table, lengths, starts, rows)
         y, fill = output_rows(out, q, self.device)
-        if not seqs.rows:
+        if not rows:
             return y
         if not seqs.sequences:
             return y.zero_() if fill else y
-        heads = q.shape[1]
         q, qp, ql, qh = heads_rows(q)
         call = ctypes.addressof(seqs)
-        shape = (seqs.sequences, seqs.rows, seqs.table_pages, starts is None, heads, q.dtype)
+        shape = (seqs.sequences, rows, seqs.table_pages, starts is None, heads, q.dtype)
         size = self._sizes.get(shape)
         if size is None:
             if len(self._sizes) >= 256:
