@@ -122,11 +122,13 @@ NO_WINDOW = 2 ** 31 - 1
 
 def launch(dev, name, *args):
     """Calls an entry point on device dev, on its current stream (the last argument)."""
-    if torch._C._cuda_getDevice() == dev.index:
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
-    else:
+    index = dev.index
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+            return launch(dev, name, *args)
+    status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, name)
 
 
 def no_grad_rows(*tensors):
@@ -158,10 +160,12 @@ def heads_rows(t, below=2 ** 63):
     """(tensor to keep alive, pointer, row stride, head stride) of rows [n, heads, dim] as the kernels read them: in place
     where the channels are contiguous, rows and heads start at 16-byte addresses and the row stride is less than `below`, else
     from a contiguous copy."""
-    unit = 16 // t.itemsize
     n, heads, dim = t.shape
-    ld, hs, one = t.stride()
     p = t.data_ptr()
+    if n > 1 and heads > 1 and t.is_contiguous() and not p % 16:
+        return t, p, heads * dim, dim
+    unit = 16 // t.itemsize
+    ld, hs, one = t.stride()
     if n == 1:  # (the stride of a dimension of one entry means nothing)
         ld = 0
     if heads == 1:
