@@ -77,10 +77,11 @@ __device__ __forceinline__ int wave_sum(int v) {
 }
 
 // The tile of workgroup `id`. Workgroups reach the 8 XCDs in turn. Where heads divide by 8, XCD x takes the heads x heads / 8 .. of
-// every sequence, so all XCDs have the same work and the tiles that share keys run on one XCD's L2; otherwise it takes every
-// eighth tile. The tiles of 64 sequences come in the order of their last query, latest first: none sees fewer keys than one after it,
-// and those that run together take about as long (workgroups start in order, and one that no CU of the next shader engine has room
-// for holds up all behind it). 16 sequences of up to 2048 tokens, 8 heads of 64, window 1024: 53 us, sequence by sequence 61.
+// every sequence, so all XCDs have the same work and the tiles that share keys run on one XCD's L2 (12000 tokens, 16 heads over 4
+// of 128: 591 us, every eighth tile 614); otherwise it takes every eighth tile. The tiles of 64 sequences come in the order of their
+// last query, latest first: none sees fewer keys than one after it, and those that run together take about as long (workgroups
+// start in order, and one that no CU of the next shader engine has room for holds up all behind it). 16 sequences of up to 2048
+// tokens, 8 heads of 64, window 1024: 50 us, sequence by sequence 61.
 template <int BQ>
 __device__ Tile find_tile(const SinkArgs& a, int id) {
   const int lane = threadIdx.x & 63, x = id & 7;
