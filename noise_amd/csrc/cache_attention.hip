@@ -20,7 +20,7 @@
 // tiles, kv head by kv head, form one line, and each of the workgroups that fill the GPU once takes an equal stretch of it:
 // every workgroup has the same to do whatever the lengths. A stretch may hold the end of one tile, whole tiles and
 // the beginning of another; the waves join in LDS, and where a tile is spread over several workgroups their sums meet in a second
-// kernel, in order (the same bits every time). Tables that name few keys go without it: a workgroup a tile.
+// kernel, in order (the same bits every time). Tables that name few keys, and very many sequences, go without it: a workgroup a tile.
 #include <type_traits>
 
 #include "common.h"
@@ -72,7 +72,7 @@ struct Plan {
   int group;        // query heads of a kv head
   int block_shift;  // log2 of a block's keys
   int cap;          // positions that a table names
-  int groups;       // workgroups that share the line, or 0: a workgroup a tile
+  int groups;       // workgroups that share the line, or 0: a workgroup a tile (and a number without one)
   int waves;        // of a workgroup: the blocks of a round
 };
 
@@ -121,7 +121,7 @@ __device__ __forceinline__ Cut cut_of(const Sequences& s, const Plan& p, int win
 struct Line {
   int units, share;
 };
-// A tile on the line of its kv head: `at` its first round, `rounds` their number; or, without a line, `at` its number.
+// A tile; on the line of its kv head `at` is its first round, `rounds` their number.
 struct Work {
   int b, s0, m, len, tile, rounds, at;
   bool found;
@@ -165,14 +165,14 @@ __device__ Work find_work(const Sequences& s, const Plan& p, int window, int sin
   for (int b0 = 0; b0 < s.n; b0 += 64) {
     int s0;
     Cut c;
-    if (p.groups && s.n <= 64) {
+    if (s.n <= 64) {
       s0 = kept.s0[lane];
       c = Cut{kept.m[lane], kept.len[lane], kept.blocks[lane], kept.tiles[lane], false};
     } else {
       c = cut_of(s, p, window, sinks, b0 + lane, s0);
       if (__any(c.bad)) return w;
     }
-    const int each = p.groups ? rounds_of(p, c) : 1;
+    const int each = rounds_of(p, c);
     const int mine = c.tiles * each;
     int upto = mine;
     for (int o = 1; o < 64; o <<= 1) {
@@ -196,6 +196,39 @@ __device__ Work find_work(const Sequences& s, const Plan& p, int window, int sin
     }
     base += uniform(upto, 63);
   }
+  return w;
+}
+
+// Tile `i` of a kv head without a line: of up to 64 sequences without gaps (the workgroups with nothing to do come last: among the
+// others, they would leave CUs idle beside CUs with two tiles: 5 rows of each of 32 sequences 24.8 us, so 15.1), of more by
+// first_tile's numbers. Whole waves.
+__device__ Work tile_of(const Sequences& s, const Plan& p, int i) {
+  const int lane = threadIdx.x & 63, each = (p.group + RT - 1) / RT;
+  Work w{};
+  if (!s.starts) {
+    w.b = i / each;
+    w.tile = i % each;
+  } else if (s.n <= 64) {
+    const int lo = lane < s.n ? min(max(s.starts[lane], 0), s.rows) : 0, hi = lane < s.n ? min(max(s.starts[lane + 1], 0), s.rows) : 0;
+    const int tiles = (max(hi - lo, 0) * p.group + RT - 1) / RT;
+    int upto = tiles;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += t;
+    }
+    const unsigned long long hits = __ballot(i < upto);
+    if (!hits || __any(hi < lo)) return w;
+    w.b = __builtin_ctzll(hits);
+    w.tile = i - uniform(upto - tiles, w.b);
+  } else {
+    w.b = last_with(s.n - 1, [&](int b) { return first_tile(s, b, p.group, RT) <= i; });
+    w.tile = i - first_tile(s, w.b, p.group, RT);
+  }
+  if (w.b >= s.n) return w;
+  w.s0 = s.starts ? min(max(s.starts[w.b], 0), s.rows) : w.b;
+  w.m = s.starts ? min(max(s.starts[w.b + 1], 0), s.rows) - w.s0 : 1;
+  w.len = max(s.lengths[w.b], 0);
+  w.found = w.tile >= 0 && w.m > 0 && w.tile < (w.m * p.group + RT - 1) / RT;
   return w;
 }
 
@@ -250,8 +283,8 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : resident(DIM, FMT, F16,
   asm volatile("" : "+v"(tid));  // (opaque: what a lane derives from it would be kept in registers over the loop)
   const int lane = tid & 63, r16 = lane & 15, grp = lane >> 4;
   const int kh = g.p.groups ? unit / line.units : blockIdx.x % c.kv_heads;
-  const Work w = find_work(s, g.p, g.a.window, g.a.sinks, g.p.groups ? unit - kh * line.units : blockIdx.x / c.kv_heads, -1, 0,
-                           kept);
+  const Work w = g.p.groups ? find_work(s, g.p, g.a.window, g.a.sinks, unit - kh * line.units, -1, 0, kept)
+                            : tile_of(s, g.p, blockIdx.x / c.kv_heads);
   if (!w.found) return;
   const int G_ = g.p.group, f0 = w.tile * RT, fn = min(RT, w.m * G_ - f0), back = w.len - w.m;
   const int p0 = back + f0 / G_, p1 = back + (f0 + fn - 1) / G_;  // positions of the tile's first and last row
@@ -674,15 +707,19 @@ Shape shape_of(const Cache& c, const Sequences& s, const AttendArgs& a) {
   const long fill = (long)resident(c.dim, c.format, a.type == ROWS_F16, wide_pages(c), s.starts) * num_cus();
   // A workgroup a tile, and no second kernel, where a tile sees so few keys that this costs no more than sharing them out (a
   // round takes about 1.4 us): 11 blocks of 8 heads on eight waves 8.2 us, shared 7.3 + 4.4; 64 sequences of 33 blocks 20.8,
-  // shared 23.8 + 4.8; 8 drafts of each of 32 sequences in windows of 2048 keys 15.1, shared 15.8 + 5.8; but one sequence of 63
-  // blocks 17.5, shared 7.3 + 5.7. Also where there are many tiles, or more rounds than fit.
-  r.items = tiles;
+  // shared 23.8 + 4.8; 5 rows of each of 32 sequences in windows of 2048 keys 15.1, shared 15.8 + 5.8; but one sequence of 63
+  // blocks 17.5, shared 7.3 + 5.7.
+  // Also where there are many tiles, or more rounds than fit; with more than 64 sequences, which every workgroup would search for its
+  // stretch, a few times what fills the GPU: 512 of 8000 tokens, 8 heads, 370 us, shared 464 (3% of them of 8000, the others of 400: 80,
+  // shared 134), 1000 of 6000, one head, 84, shared 217; but 160 of up to 20000, 8 heads, 212, shared 193.
+  r.items = s.starts ? (full + s.n) * c.kv_heads : tiles;
   r.p.waves = 4;
   if (blocks <= 40 && tiles <= 2 * num_cus()) {
     r.p.waves = 8;
     return r;
   }
-  if (blocks <= 18 || (blocks <= 66 && tiles >= fill / 2) || tiles >= 32 * fill || tiles * (all + 2) > 0x3fffffffL) return r;
+  const bool many = s.n <= 64 ? tiles >= 32 * fill : tiles >= (s.n < 512 ? 2 * fill : fill / 2);
+  if (blocks <= 18 || (blocks <= 66 && tiles >= fill / 2) || many || tiles * (all + 2) > 0x3fffffffL) return r;
   const long most = tiles * ((blocks + r.p.waves - 1) / r.p.waves);
   r.items = r.p.groups = (int)(most < fill ? most : fill);
   return r;

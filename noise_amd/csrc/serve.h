@@ -65,23 +65,36 @@ int sink_attention_launch(const SinkArgs& a, hipStream_t stream);
 
 // ---------------------------------------------------------------- device helpers
 
-// The sequence that owns row i: the number of entries of starts[1 .. n] that are <= i, found by a wave 64 entries at a time
-// (one round of loads up to 64 sequences, two up to 4096). Rows of no sequence give n. Called by whole waves.
-__device__ __forceinline__ int find_sequence(const int* starts, int n, int i) {
+// The largest b in [0, n] with in(b), where in(b) holds for no b after one for which it does not (in(0) is not asked); found by a
+// wave 64 entries at a time (one round up to 64, two up to 4096). Called by whole waves.
+template <class F>
+__device__ __forceinline__ int last_with(int n, F in) {
   const int lane = threadIdx.x & 63;
   int lo = 0, hi = n;  // the answer lies in [lo, hi]
   while (hi - lo > 64) {
     const int step = (hi - lo + 63) / 64;
-    const int at = lo + (lane + 1) * step;  // probe entry `at`: starts[at] <= i means the answer is >= at
-    const unsigned long long m = __ballot(at <= hi && starts[at] <= i);
+    const int at = lo + (lane + 1) * step;
+    const unsigned long long m = __ballot(at <= hi && in(at));
     const int k = m == ~0ull ? 64 : __builtin_ctzll(~m);
     const int nlo = lo + k * step;
     hi = max(nlo, min(hi, nlo + step - 1));
     lo = nlo;
   }
   const int at = lo + lane + 1;
-  const unsigned long long m = __ballot(at <= hi && starts[at] <= i);
+  const unsigned long long m = __ballot(at <= hi && in(at));
   return lo + __builtin_popcountll(m);
+}
+
+// The sequence that owns row i: the number of entries of starts[1 .. n] that are <= i. Rows of no sequence give n.
+__device__ __forceinline__ int find_sequence(const int* starts, int n, int i) {
+  return last_with(n, [&](int b) { return starts[b] <= i; });
+}
+
+// Tiles of `per` units (a row is `mul` of them) that begin with every sequence are numbered with gaps, so that a sequence's first
+// number follows from its start alone: rows mul / per + b, at least the tiles of all sequences in front (and of all, in front of
+// sequence n: the numbers' limit).
+__device__ __forceinline__ int first_tile(const Sequences& s, int b, int mul, int per) {
+  return (int)((long)min(max(s.starts[b], 0), s.rows) * mul / per) + b;
 }
 
 constexpr int POSITIONS = 0x7fffff00;  // a position's limit: sums with a block's keys stay within an int
@@ -99,6 +112,15 @@ __device__ __forceinline__ long slot_of(const Cache& c, const Sequences& s, int 
 __device__ __forceinline__ int uniform(int x, int k = 0) { return __builtin_amdgcn_readlane(x, k); }
 __device__ __forceinline__ long uniform(long x, int k = 0) {
   return (long)((unsigned long long)(unsigned)uniform((int)(x >> 32), k) << 32 | (unsigned)uniform((int)x, k));
+}
+
+// The sum over a wave's lanes.
+__device__ __forceinline__ int wave_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, DPP_QUAD_XOR1, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, DPP_QUAD_XOR2, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, DPP_ROW_HALF_MIRROR, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, DPP_ROW_MIRROR, 0xF, 0xF, false);
+  return uniform(v) + uniform(v, 16) + uniform(v, 32) + uniform(v, 48);
 }
 
 // Zeroes the rows of no sequence, in front of the first one and behind the last: workgroup `part` of `parts` of nth threads.

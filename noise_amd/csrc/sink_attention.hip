@@ -67,15 +67,6 @@ struct Tile {
   bool found;
 };
 
-// The sum over a wave's lanes.
-__device__ __forceinline__ int wave_sum(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, DPP_QUAD_XOR1, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, DPP_QUAD_XOR2, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, DPP_ROW_HALF_MIRROR, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, DPP_ROW_MIRROR, 0xF, 0xF, false);
-  return uniform(v) + uniform(v, 16) + uniform(v, 32) + uniform(v, 48);
-}
-
 // The tile of workgroup `id`. Workgroups reach the 8 XCDs in turn. Where heads divide by 8, XCD x takes the heads x heads / 8 .. of
 // every sequence, so all XCDs have the same work and the tiles that share keys run on one XCD's L2 (12000 tokens, 16 heads over 4
 // of 128: 591 us, every eighth tile 614); otherwise it takes every eighth tile. The tiles of 64 sequences come in the order of their
@@ -90,38 +81,37 @@ __device__ Tile find_tile(const SinkArgs& a, int id) {
   const int at = even ? id >> 3 : id, turn = at / per, h = at % per;
   Tile t{};
   // (all counts are below the grid's size)
-  int base = 0;
-  for (int b0 = 0; b0 < a.n; b0 += 64) {
-    const int b = b0 + lane;
-    int s0 = 0, m = 0;
-    if (b < a.n) {
-      s0 = a.starts ? min(max(a.starts[b], 0), a.rows) : b * a.T;
-      m = a.starts ? min(max(a.starts[b + 1], 0), a.rows) - s0 : a.T;
-    }
-    if (__any(m < 0)) return t;  // starts that decrease: nothing more is found
-    const int tiles = (m + BQ - 1) / BQ, all = wave_sum(tiles);
-    if (turn - base < all) {
-      // the level, a tile's number in its sequence: the last from which on there are more tiles than come before this one
-      int level = 0, over = (a.rows + BQ - 1) / BQ, before = 0;
-      while (over - level > 1) {
-        const int mid = (level + over) >> 1, from = wave_sum(max(tiles - mid, 0));
-        if (from > turn - base)
-          level = mid;
-        else
-          over = mid, before = from;
-      }
-      const unsigned long long has = __ballot(tiles > level);
-      const int nth = __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
-      const int k = __builtin_ctzll(__ballot((tiles > level) & (nth == turn - base - before)));
-      t.found = true;
-      t.s0 = uniform(s0, k);
-      t.m = uniform(m, k);
-      t.q0 = level * BQ;
-      t.h = even ? x * per + h : h;
-      return t;
-    }
-    base += all;
+  const Sequences rows{nullptr, 0, 0, nullptr, a.starts, a.n, a.rows};
+  const int each = (a.T + BQ - 1) / BQ;
+  auto first = [&](int b) { return a.starts ? first_tile(rows, b, 1, BQ) : b * each; };
+  const int b0 = a.n <= 64 ? 0 : 64 * last_with((a.n - 1) / 64, [&](int c) { return first(64 * c) <= turn; });
+  const int base = first(b0);
+  const int b = b0 + lane;
+  int s0 = 0, m = 0;
+  if (b < a.n) {
+    s0 = a.starts ? min(max(a.starts[b], 0), a.rows) : b * a.T;
+    m = a.starts ? min(max(a.starts[b + 1], 0), a.rows) - s0 : a.T;
   }
+  if (__any(m < 0) || turn < base) return t;  // (starts that decrease: nothing is found)
+  const int tiles = (m + BQ - 1) / BQ;
+  if (turn - base >= wave_sum(tiles)) return t;
+  // the level, a tile's number in its sequence: the last from which on there are more tiles than come before this one
+  int level = 0, over = (a.rows + BQ - 1) / BQ, before = 0;
+  while (over - level > 1) {
+    const int mid = (level + over) >> 1, from = wave_sum(max(tiles - mid, 0));
+    if (from > turn - base)
+      level = mid;
+    else
+      over = mid, before = from;
+  }
+  const unsigned long long has = __ballot(tiles > level);
+  const int nth = __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
+  const int k = __builtin_ctzll(__ballot((tiles > level) & (nth == turn - base - before)));
+  t.found = true;
+  t.s0 = uniform(s0, k);
+  t.m = uniform(m, k);
+  t.q0 = level * BQ;
+  t.h = even ? x * per + h : h;
   return t;
 }
 
@@ -391,9 +381,9 @@ int sink_attention_launch(const SinkArgs& a, hipStream_t stream) {
     return NOISE_EINVAL;
   // (byte strides of 24 bits: offsets inside a 64-key block are 24-bit products)
   if (a.k.ld >= (1 << 23) || a.v.ld >= (1 << 23)) return NOISE_ENOTSUP;
-  // tiles: of queries, at most one begun by every sequence beside the full ones; the GPU counts them
+  // tiles' numbers: the full ones and one more for every sequence; the GPU finds which are tiles
   auto groups = [&](int bq) {
-    const long tiles = a.starts ? a.rows / bq + (a.n < a.rows ? a.n : a.rows) : (long)a.n * ((a.T + bq - 1) / bq);
+    const long tiles = a.starts ? a.rows / bq + a.n : (long)a.n * ((a.T + bq - 1) / bq);
     return a.heads % 8 == 0 ? tiles * a.heads : (tiles * a.heads + 7) / 8 * 8;
   };
   // Tiles of 64 queries where those of 128 leave the GPU empty for much of the time, and two groups of waves where those do too (8

@@ -207,6 +207,10 @@ def test_many_prompts():
     q, k, v = (rows(g, sum(lens), 1, 64, BF16) for _ in range(3))
     y, terms = prompt_reference(q, k, v, lens, None, 0)
     check(ops.sink_attention(q.to(DEV), k.to(DEV), v.to(DEV), i32(starts_of(lens))), y, terms, BF16, BF16)
+    for heads in (1, 8):
+        x = rows(g, 900, heads, 64, BF16).to(DEV)  # (sequences of one length, with and without starts)
+        want = ops.sink_attention(x, x, x, i32(range(0, 901, 3)), window=1)
+        assert torch.equal(ops.sink_attention(*[x.view(300, 3, heads, 64)] * 3, window=1).view(900, heads, 64), want)
 
 
 def test_prompt_types_and_shapes_are_refused():
@@ -426,6 +430,20 @@ def test_attention_over_the_cache(case):
     st = i32(starts_of(m)) if new else None
     got = f.cache.attend(q.to(DEV), f.table, f.lengths, st, window=window, sinks=sinks)
     check(got, y, terms, dtype, P_CACHE if dtype == BF16 else None)
+
+
+@pytest.mark.parametrize('step,heads,kv', [(True, 2, 2), (False, 20, 1)])
+def test_many_cached_sequences(step, heads, kv):
+    """More sequences than two search rounds cover, many empty; and on tables long enough for the rows to be shared out."""
+    g = torch.Generator().manual_seed(50)
+    for n, top, pages in ((5000, 40, 3), (300, 40, 300)):
+        lens = [int(x) for x in torch.randint(0, top, (n,), generator=g)]
+        new = [1] * n if step else [int(x) for x in torch.randint(0, 3, (n,), generator=g)]
+        f = Filled(lens, kv, 64, 'fp8', 16, seed=51)
+        q = rows(g, sum(new), heads, 64, BF16)
+        y, terms = attend_reference(f, q, new, None, 0)
+        table = torch.cat((f.table, torch.zeros(n, pages - f.table.shape[1], device=DEV, dtype=torch.int32)), 1)
+        check(f.cache.attend(q.to(DEV), table, f.lengths, None if step else i32(starts_of(new))), y, terms, BF16, P_CACHE)
 
 
 def test_cache_scale_and_large_scores():
